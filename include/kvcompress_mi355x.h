@@ -393,6 +393,85 @@ int kvc_physical_slot_mapping(kvc_stream_t stream, int num_reqs, const int32_t* 
 int kvc_shift_lengths(kvc_stream_t stream, void* seq_lens, int elem_bytes, const int64_t* request_offsets,
                       int num_reqs);
 
+/* ------------------------------------------- model step on a paged cache -- */
+
+/* Tables of one step from its requests' lengths: request r has computed_tokens[r]
+ * tokens behind it (semantic count) and brings new_tokens[r] (negative counts as
+ * 0); request_offsets[r] = semantic - physical length (NULL: none); its
+ * scheduler pages of page_tokens tokens (a multiple of 128) are
+ * block_ids[block_offsets[r] .. block_offsets[r+1]).  Written, for r < n_seq:
+ *   query_start_loc[r], [n_seq]: tokens before request r, and all (int32)
+ *   seq_lens[r] = computed + new - offset, at least 0 (int32)
+ *   positions[t] = computed + i of token t = query_start_loc[r] + i (int64)
+ *   block_table[r][j], j < max_blocks: 128-token page j, for j*128 <
+ *     seq_lens[r]; -1 behind it and where the ragged row has no page (int32)
+ *   slot_mapping[t] = page(p/128)*128 + p%128 of p = positions[t] - offset; -1
+ *     where p is negative or has no page in the table (int64)
+ * Tokens t >= query_start_loc[n_seq] (padding) get slot -1 and position 0.
+ * Tokens past num_tokens are dropped: the request they belong to ends there and
+ * the ones behind it bring none.  max_query_len sizes the launch only.  The
+ * inputs may not overlap the outputs.  No counterpart in the reference, whose
+ * host builds these (kvc_physical_slot_mapping replaces its hook). */
+int kvc_step_tables(kvc_stream_t stream, int n_seq, const int32_t* computed_tokens, const int32_t* new_tokens,
+                    const int64_t* request_offsets, const int64_t* block_ids, const int64_t* block_offsets,
+                    int page_tokens, int max_query_len, int64_t num_tokens, int max_blocks, int64_t block_table_stride,
+                    int32_t* query_start_loc, int32_t* seq_lens, int64_t* positions, int64_t* slot_mapping,
+                    int32_t* block_table);
+
+/* Rotary positions of a step's tokens, and their keys and values in the cache:
+ * for frequency f < F = rotary_dim/2 and its axis x,
+ *   theta = positions[x*position_stride + t] * omega[f]   (float64, as cos/sin float32)
+ *   (a, b) -> (a*cos - b*sin, a*sin + b*cos)
+ * on dims (f, F+f) (KVC_ROPE_HALF) or (2f, 2f+1) (KVC_ROPE_INTERLEAVED), in
+ * float32, rounded once; dims from rotary_dim on pass through.  sections_host
+ * (n_axes <= 4 host ints adding up to F) shares the frequencies among the axes:
+ * runs in axis order, or (cycled) f%n_axes while f/n_axes < that axis's
+ * section and axis 0 for the rest.  Element (t, h, d) of q is at
+ * q[t*q_token_stride + h*q_head_stride + d], k and v likewise.  Turned queries
+ * go to q_out (which may be q itself with the same strides, else may not overlap
+ * it), turned keys and the values to row slot_mapping[t] of the cache
+ * ([num_pages][128][kv_heads][head_dim]); slots outside [0, num_pages*128) store
+ * nothing.  A slot may be named by one token only.  head_dim <= 1024,
+ * rotary_dim <= 512.  No counterpart in the reference (its host's model does it). */
+int kvc_rotate_and_store(kvc_stream_t stream, int dtype, int rope_style, int64_t num_tokens, int heads, int kv_heads,
+                         int head_dim, int rotary_dim, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                         const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                         int64_t v_token_stride, int64_t v_head_stride, const int64_t* positions,
+                         int64_t position_stride, int n_axes, const int* sections_host, int cycled, const float* omega,
+                         const int64_t* slot_mapping, void* q_out, int64_t out_token_stride, int64_t out_head_stride,
+                         void* k_cache, void* v_cache, int64_t num_pages, int64_t page_stride);
+
+/* Attention of a step's new tokens over the paged cache, which holds their own
+ * keys and values already.  Request r owns tokens query_start_loc[r] ..
+ * query_start_loc[r+1] of q; with `new` of them and len = seq_lens[r] (cached
+ * tokens, the new ones among them) token i is at place p = len - new + i and
+ *   out = sum_j softmax_j(scale * q.k_j) v_j
+ *   over keys j <= p with (window == 0 or p - j < window or j < sinks).
+ * Places are physical: after a compaction the window counts kept tokens, and
+ * sinks are the first kept ones (protected_prefix keeps a prompt's first).  Keys
+ * in pages outside [0, num_pages) or past max_blocks are not seen; rows that see
+ * no key give zeros; what a key's row holds never reaches a row that does not
+ * see it, NaN and infinities included.  Query head h*qpk + g belongs to KV head
+ * h.  Element (t, head, d) of q and out at t*token_stride + head*head_stride + d;
+ * strides in multiples of 8 elements, every pointer 16-byte aligned, head_dim a
+ * multiple of 8 up to 256.  max_query_len must bound every request's new tokens
+ * (rows of longer ones may be left out); max_seq_len sizes the launch only.
+ * scale is positive.  out may not overlap q; its rows outside every request are
+ * left as they were.  Scores, softmax and sums are float32; the weights of
+ * requests with more than 32 rows (new*qpk) are rounded to the cache's type
+ * before the product with V.  Results are the same on every run of a shape.
+ * workspace: kvc_attend_workspace_bytes of the same sizes (0 for sizes that are
+ * refused), any contents; calls that overlap in time need one each.
+ * No counterpart in the reference (its host's attention backend reads the cache). */
+size_t kvc_attend_workspace_bytes(int kv_heads, int qpk, int head_dim, int n_seq, int64_t num_tokens,
+                                  int max_query_len, int max_seq_len);
+int kvc_attend_paged(kvc_stream_t stream, int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                     const void* k_cache, const void* v_cache, int64_t num_pages, int64_t page_stride, int kv_heads,
+                     int qpk, int head_dim, int n_seq, int64_t num_tokens, const int32_t* query_start_loc,
+                     const int32_t* seq_lens, const int32_t* block_table, int64_t block_table_stride, int max_blocks,
+                     int max_query_len, int max_seq_len, float scale, int window, int sinks, void* out,
+                     int64_t out_token_stride, int64_t out_head_stride, void* workspace, size_t workspace_bytes);
+
 /* ----------------------------------------------------------- calibration -- */
 
 /* Query statistics of one layer's pre-RoPE query projections, accumulated over

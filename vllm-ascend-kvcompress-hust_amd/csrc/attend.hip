@@ -1,0 +1,148 @@
+// Entry of the attention over a paged cache: checks, launch sizes, workspace.
+
+#include <math.h>
+
+#include "attend_internal.h"
+
+namespace kvc {
+namespace {
+
+constexpr int kCompute = 256;  // compute units of the device
+
+// How a call is launched; the workspace query and the call agree by sharing it.
+struct AttendPlan {
+  int row_tiles;    // 16-row tiles a request of the few-rows kernel has at most; 0: kernel not needed
+  int workgroups;   // of the few-rows kernel
+  int64_t tiles;    // 128-row tiles of the many-rows kernel; 0: kernel not needed
+  int splits;       // of their keys
+  int sequences;    // requests of one few-rows launch
+  size_t bytes;     // workspace
+};
+
+AttendPlan make_plan(int kv_heads, int qpk, int head_dim, int n_seq, int64_t num_tokens, int max_query_len, int max_seq_len) {
+  AttendPlan p = {};
+  const int dim = padded_dim(head_dim);
+  const int64_t most_rows = static_cast<int64_t>(max_query_len) * qpk;
+  const int64_t pages = ceil_div(max_seq_len > 0 ? max_seq_len : 1, kBlockSize);
+  size_t few = 0, many = 0;
+  if (qpk <= kFewRows * kFewTilesMost) {
+    p.row_tiles = most_rows <= kFewRows ? 1 : kFewTilesMost;
+    p.sequences = n_seq < kFewSequences ? n_seq : kFewSequences;
+    const int64_t bound = static_cast<int64_t>(p.sequences) * kv_heads * pages;
+    // Workgroups that fit the device at once: 3 or 2 a compute unit by their LDS.
+    const int64_t resident = kCompute * (dim <= 128 ? 3 : 2);
+    p.workgroups = static_cast<int>(bound < resident ? bound : resident);
+    few = static_cast<size_t>(p.workgroups) * (16 + 8 * piece_floats(kFewRows * p.row_tiles, dim));
+  }
+  if (most_rows > kFewRows * p.row_tiles) {
+    p.tiles = num_tokens * qpk / kManyRows + n_seq;
+    // Two workgroups a compute unit are wanted; a split is not worth fewer than 512 keys.
+    const int64_t filled = ceil_div(num_tokens * qpk, kManyRows) * kv_heads;
+    int64_t splits = filled >= 2 * kCompute ? 1 : ceil_div(2 * kCompute, filled);
+    const int64_t by_keys = ceil_div(pages * kBlockSize, 512), by_space = 4096 / (p.tiles * kv_heads);
+    if (splits > by_keys) splits = by_keys;
+    if (splits > by_space) splits = by_space;
+    p.splits = splits < 1 ? 1 : static_cast<int>(splits);
+    if (p.splits > 1) many = static_cast<size_t>(p.tiles) * kv_heads * p.splits * piece_floats(kManyRows, dim) * 4;
+  }
+  p.bytes = few > many ? few : many;
+  if (p.bytes == 0) p.bytes = 16;
+  return p;
+}
+
+bool good_shape(int kv_heads, int qpk, int head_dim, int n_seq, int64_t num_tokens, int max_query_len, int max_seq_len) {
+  return kv_heads > 0 && qpk > 0 && kv_heads <= 1024 && qpk <= 1024 && head_dim > 0 && head_dim % 8 == 0 && padded_dim(head_dim) &&
+         n_seq >= 0 && num_tokens >= 0 && num_tokens < (1 << 24) && n_seq < (1 << 24) && max_query_len >= 0 && max_seq_len >= 0;
+}
+
+}  // namespace
+}  // namespace kvc
+
+using namespace kvc;
+
+extern "C" size_t kvc_attend_workspace_bytes(int kv_heads, int qpk, int head_dim, int n_seq, int64_t num_tokens,
+                                             int max_query_len, int max_seq_len) {
+  if (!good_shape(kv_heads, qpk, head_dim, n_seq, num_tokens, max_query_len, max_seq_len)) return 0;
+  return make_plan(kv_heads, qpk, head_dim, n_seq, num_tokens, max_query_len, max_seq_len).bytes;
+}
+
+extern "C" int kvc_attend_paged(kvc_stream_t stream, int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                                const void* k_cache, const void* v_cache, int64_t num_pages, int64_t page_stride, int kv_heads,
+                                int qpk, int head_dim, int n_seq, int64_t num_tokens, const int32_t* query_start_loc,
+                                const int32_t* seq_lens, const int32_t* block_table, int64_t block_table_stride, int max_blocks,
+                                int max_query_len, int max_seq_len, float scale, int window, int sinks, void* out,
+                                int64_t out_token_stride, int64_t out_head_stride, void* workspace, size_t workspace_bytes) {
+  if (dtype != KVC_DTYPE_BF16 && dtype != KVC_DTYPE_FP16) return fail(KVC_EINVAL, "kvc_attend_paged: dtype must be bf16 or fp16");
+  if (!good_shape(kv_heads, qpk, head_dim, n_seq, num_tokens, max_query_len, max_seq_len))
+    return fail(KVC_EINVAL,
+                "kvc_attend_paged: bad sizes (head_dim %d must be a multiple of 8 up to 256; kv_heads %d, qpk %d at most 1024; "
+                "n_seq %d, num_tokens %lld below 2^24)",
+                head_dim, kv_heads, qpk, n_seq, static_cast<long long>(num_tokens));
+  if (num_pages < 0 || page_stride < static_cast<int64_t>(kBlockSize) * kv_heads * head_dim || page_stride % 8)
+    return fail(KVC_EINVAL, "kvc_attend_paged: page_stride must be a multiple of 8 elements and at least one page");
+  if (max_blocks < 0 || max_blocks >= (1 << 23) || block_table_stride < max_blocks)
+    return fail(KVC_EINVAL, "kvc_attend_paged: max_blocks must be below 2^23 and at most block_table_stride");
+  if (!(scale > 0.0f) || !isfinite(scale)) return fail(KVC_EINVAL, "kvc_attend_paged: scale must be positive and finite");
+  if (window < 0 || sinks < 0) return fail(KVC_EINVAL, "kvc_attend_paged: window and sinks must be non-negative");
+  if (n_seq == 0 || num_tokens == 0 || max_query_len == 0) return 0;
+  if (!q || !out || !query_start_loc || !seq_lens || (max_blocks > 0 && !block_table) || (num_pages > 0 && (!k_cache || !v_cache)))
+    return fail(KVC_EINVAL, "kvc_attend_paged: null pointer");
+  const uintptr_t bases = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(k_cache) |
+                          reinterpret_cast<uintptr_t>(v_cache) | reinterpret_cast<uintptr_t>(workspace);
+  if (bases % 16 || (q_token_stride | q_head_stride | out_token_stride | out_head_stride) % 8)
+    return fail(KVC_EINVAL, "kvc_attend_paged: pointers must be 16-byte aligned and strides multiples of 8 elements");
+  const AttendPlan plan = make_plan(kv_heads, qpk, head_dim, n_seq, num_tokens, max_query_len, max_seq_len);
+  if (!workspace || workspace_bytes < plan.bytes)
+    return fail(KVC_EINVAL, "kvc_attend_paged: workspace too small (%zu of %zu bytes)", workspace_bytes, plan.bytes);
+  if (plan.tiles * kv_heads * plan.splits >= (1ll << 31))
+    return fail(KVC_EINVAL, "kvc_attend_paged: too many rows for one launch");
+
+  AttendArgs a = {};
+  a.q = static_cast<const uint16_t*>(q);
+  a.out = static_cast<uint16_t*>(out);
+  a.k = static_cast<const uint16_t*>(k_cache);
+  a.v = static_cast<const uint16_t*>(v_cache);
+  a.q_token_stride = q_token_stride;
+  a.q_head_stride = q_head_stride;
+  a.out_token_stride = out_token_stride;
+  a.out_head_stride = out_head_stride;
+  a.num_pages = num_pages;
+  a.page_stride = page_stride;
+  a.table_stride = block_table_stride;
+  a.num_tokens = num_tokens;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.kv_heads = kv_heads;
+  a.qpk = qpk;
+  a.head_dim = head_dim;
+  a.max_blocks = max_blocks;
+  a.window = window < (1 << 30) ? window : 0;  // the table covers fewer keys than that
+  a.sinks = sinks;
+  a.few_rows = kFewRows * plan.row_tiles;
+  const hipStream_t st = as_stream(stream);
+  const bool f16 = dtype == KVC_DTYPE_FP16;
+  if (plan.row_tiles) {
+    a.header = static_cast<int32_t*>(workspace);
+    a.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + 16 * static_cast<size_t>(plan.workgroups));
+    // Tile numbers are 32-bit: requests x heads x pages of a launch stay below 2^30.
+    const int64_t each = static_cast<int64_t>(kv_heads) * (max_blocks > 0 ? max_blocks : 1);
+    if (each > (1 << 30)) return fail(KVC_EINVAL, "kvc_attend_paged: kv_heads x max_blocks must be at most 2^30");
+    int64_t chunk = (1 << 30) / each;
+    if (chunk > kFewSequences) chunk = kFewSequences;
+    for (int64_t base = 0; base < n_seq; base += chunk) {
+      a.n_seq = static_cast<int>(n_seq - base < chunk ? n_seq - base : chunk);
+      a.start = query_start_loc + base;
+      a.seq_lens = seq_lens + base;
+      a.table = block_table + base * block_table_stride;
+      if (int rc = launch_attend_few(st, f16, a, plan.workgroups, plan.row_tiles)) return rc;
+    }
+  }
+  if (plan.tiles) {
+    a.n_seq = n_seq;
+    a.start = query_start_loc;
+    a.seq_lens = seq_lens;
+    a.table = block_table;
+    a.partial = static_cast<float*>(workspace);
+    if (int rc = launch_attend_many(st, f16, a, plan.tiles, plan.splits)) return rc;
+  }
+  return 0;
+}

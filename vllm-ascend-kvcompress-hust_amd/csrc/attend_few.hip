@@ -1,0 +1,444 @@
+// Attention of requests with few rows (single tokens, a few drafted ones):
+// every key is read once for at most 32 query rows, so the cache's bytes bound
+// it.  Work is (request, KV head, page) tiles in that order, split evenly over
+// the workgroups whatever the requests' lengths, so one long request beside
+// short ones takes no longer than its share.  A workgroup's range may begin or
+// end inside a (request, head): those pieces go to the workspace and a second
+// launch joins them; a (request, head) inside one range is written at once.
+//
+// A workgroup's four waves take 32 keys each of a page.  Scores are formed
+// transposed (S^T = K Q^T, 16x16x32): a lane then holds one query row's scores,
+// and the same registers are the right operand of O^T = V^T P^T once keys are
+// numbered as they lie in them: slot (lane/16, j) of a product's 32 keys is key
+// 16*(j/4) + 4*(lane/16) + j%4.  K goes from memory to registers in operand
+// order; V passes through the wave's own LDS, where ds_read_b64_tr_b16 turns
+// rows into columns.
+
+#include "attend_internal.h"
+
+namespace kvc {
+namespace {
+
+constexpr int kFewThreads = 256;
+constexpr int kFewWaves = 4;
+constexpr int kSliceKeys = 32;  // keys of a wave's slice of a page
+
+// LDS row length of V (a power of two of 16-byte chunks) and the place of a
+// chunk: the 32-byte pairs of eight rows' same columns fall on different banks.
+template <int DP>
+struct FewLayout {
+  static constexpr int kRow = DP <= 64 ? 64 : (DP <= 128 ? 128 : 256);
+  __device__ __forceinline__ static int at(int row, int chunk) {
+    const int turn = kRow == 64 ? (row >> 1) & 3 : row & 7;
+    return row * kRow + ((chunk ^ (2 * turn)) << 3);
+  }
+};
+
+// Waves a SIMD: as many as the registers of a variant's outputs, queries and
+// one slice's K and V leave room for.
+constexpr int few_waves(int dp, int nq) { return dp <= 64 ? (nq == 1 ? 4 : 3) : (dp <= 128 ? (nq == 1 ? 3 : 2) : (nq == 1 ? 2 : 1)); }
+
+template <bool F16, int DP, int NQ>
+__global__ __launch_bounds__(kFewThreads, few_waves(DP, NQ)) void attend_few_kernel(AttendArgs a) {
+  typedef AttendElem<F16> E;
+  typedef typename E::vec vec_t;
+  constexpr int kSteps = DP / 32;   // 32-dim steps of K Q^T
+  constexpr int kBlocks = DP / 16;  // 16-dim blocks of the output
+  constexpr int kChunks = DP / 8;   // 16-byte chunks of a row
+  constexpr int kLoads = kSliceKeys * kChunks / 64;
+  constexpr int kRows = 16 * NQ;
+  typedef FewLayout<DP> Layout;
+  __shared__ __attribute__((aligned(16))) uint16_t v_stage[kFewWaves][kSliceKeys * Layout::kRow];
+  __shared__ int before[kFewSequences + 1];
+  __shared__ float wave_m[kFewWaves][kRows], wave_l[kFewWaves][kRows];
+  __shared__ int wave_sum[kFewWaves];
+
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, group = lane >> 4;
+
+  // Tiles before each request.
+  if (tid == 0) before[0] = 0;
+  int carried = 0;
+  for (int base = 0; base < a.n_seq; base += kFewThreads) {
+    const int r = base + tid;
+    int tiles = 0;
+    if (r < a.n_seq) {
+      const Request s = request_of(a, r);
+      if (s.fresh > 0 && static_cast<int64_t>(s.fresh) * a.qpk <= a.few_rows) {
+        tiles = tile_range<kBlockShift>(a, s, s.len - s.fresh, s.len - 1).count();
+        tiles = (tiles < 1 ? 1 : tiles) * a.kv_heads;  // a request without keys is written by one empty tile a head
+      }
+    }
+    int sum = tiles;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int up = __shfl_up(sum, d);
+      if (lane >= d) sum += up;
+    }
+    if (lane == 63) wave_sum[wave] = sum;
+    __syncthreads();
+    int add = carried, all = 0;
+#pragma unroll
+    for (int w = 0; w < kFewWaves; ++w) {
+      if (w < wave) add += wave_sum[w];
+      all += wave_sum[w];
+    }
+    if (r < a.n_seq) before[r + 1] = sum + add;
+    carried += all;
+    __syncthreads();
+  }
+  const int total = before[a.n_seq];
+  const int per = (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+  const int wg = blockIdx.x;
+  if (tid == 0) a.header[4 * wg + 2] = 0;  // no pieces to join until one begins here
+  int at = wg * per;
+  const int range_begin = at;
+  const int range_end = at + per < total ? at + per : total;
+  if (at >= range_end) return;
+
+  // The request that holds tile `at`.
+  int r = 0;
+  for (int span = 1 << 10; span; span >>= 1)
+    if (r + span < a.n_seq && before[r + span] <= at) r += span;
+
+  const int64_t row_elems = static_cast<int64_t>(a.kv_heads) * a.head_dim;
+  while (at < range_end) {
+    while (before[r + 1] <= at) ++r;
+    const Request s = request_of(a, r);
+    const TileRange pages = tile_range<kBlockShift>(a, s, s.len - s.fresh, s.len - 1);
+    const int tiles = (before[r + 1] - before[r]) / a.kv_heads;
+    const int head = (at - before[r]) / tiles;
+    const int piece_first = at - before[r] - head * tiles;
+    const int whole_begin = before[r] + head * tiles;
+    const int piece_end = whole_begin + tiles < range_end ? whole_begin + tiles : range_end;
+    const int piece_last = piece_end - whole_begin;
+    const int rows = s.fresh * a.qpk;
+    const int place0 = s.len - s.fresh;
+
+    vec_t qf[NQ][kSteps];
+    RowSight sight[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      const int m = n * 16 + col;
+      const int token = m / a.qpk, g = m - token * a.qpk;
+      const bool inside = m < rows;
+      const int place = place0 + token;
+      sight[n] = sight_of(a, s, place);
+      if (!inside) sight[n].end = 0;
+      const uint16_t* row = a.q + (s.token0 + (inside ? token : 0)) * a.q_token_stride +
+                            (head * a.qpk + (inside ? g : 0)) * a.q_head_stride;
+#pragma unroll
+      for (int st = 0; st < kSteps; ++st) {
+        const int d = st * 32 + group * 8;
+        u32x4 w = {0, 0, 0, 0};
+        if (inside && d < a.head_dim) w = *gptr(reinterpret_cast<const u32x4*>(row + d));
+        qf[n][st] = __builtin_bit_cast(vec_t, w);
+      }
+    }
+    // Keys that some row sees, and those that every row sees.
+    const int last_end = place0 + s.fresh < s.keys ? place0 + s.fresh : s.keys;
+    const int first_end = place0 + 1 < s.keys ? place0 + 1 : s.keys;
+    const int first_low = a.window ? place0 - a.window + 1 : 0;
+    const int last_low = a.window ? s.len - a.window : 0;
+
+    f32x4 acc[NQ][kBlocks];
+    float m_run[NQ], l_run[NQ];
+    // Weights of zero, and second words of any sign, turn an infinity or NaN
+    // among V into NaN for rows that do not see it.  That shows in the outputs:
+    // a wave that finds one there goes over its keys again with care.
+    for (bool careful = false;; careful = true) {
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      m_run[n] = kNegInf;
+      l_run[n] = 0.0f;
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) acc[n][b] = f32x4{0, 0, 0, 0};
+    }
+
+    for (int t = piece_first; t < piece_last; ++t) {
+      if (pages.count() == 0) break;
+      const int block = pages.tile(t);
+      const int page = a.table[r * a.table_stride + block];
+      if (page < 0 || page >= a.num_pages) continue;  // nothing of it is seen
+      const int key0 = (block << kBlockShift) + wave * kSliceKeys;
+      if (key0 >= last_end || (key0 + kSliceKeys <= first_low && key0 >= a.sinks)) continue;
+      const bool whole = key0 + kSliceKeys <= first_end && (key0 >= last_low || key0 + kSliceKeys <= a.sinks);
+      const int64_t base = page * a.page_stride + (wave * kSliceKeys) * row_elems + head * a.head_dim;
+      const uint16_t* kp = a.k + base;
+      const uint16_t* vp = a.v + base;
+
+      u32x4 kw[2][kSteps], vw[kLoads];
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int st = 0; st < kSteps; ++st) {
+          const int d = st * 32 + group * 8;
+          kw[b][st] = u32x4{0, 0, 0, 0};
+          if (d < a.head_dim) kw[b][st] = *gptr(reinterpret_cast<const u32x4*>(kp + (b * 16 + col) * row_elems + d));
+        }
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int u = i * 64 + lane, row = u / kChunks, c = u - row * kChunks;
+        vw[i] = u32x4{0, 0, 0, 0};
+        if (c * 8 < a.head_dim) vw[i] = *gptr(reinterpret_cast<const u32x4*>(vp + row * row_elems + c * 8));
+      }
+
+      f32x4 sc[NQ][2];
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          sc[n][b] = f32x4{0, 0, 0, 0};
+#pragma unroll
+          for (int st = 0; st < kSteps; ++st) sc[n][b] = E::mfma(__builtin_bit_cast(vec_t, kw[b][st]), qf[n][st], sc[n][b]);
+        }
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int u = i * 64 + lane, row = u / kChunks, c = u - row * kChunks;
+        if (key0 + row >= s.keys) vw[i] = u32x4{0, 0, 0, 0};  // behind the request: whatever the page holds
+        *reinterpret_cast<u32x4*>(&v_stage[wave][Layout::at(row, c)]) = vw[i];
+      }
+
+      vec_t hi[NQ], lo[NQ];
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        float x[8], top = kNegInf;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          x[j] = sc[n][j >> 2][j & 3] * a.scale_log2;
+          if (!whole && !sees(sight[n], a.sinks, key0 + 16 * (j >> 2) + 4 * group + (j & 3))) x[j] = kNegInf;
+          top = fmaxf(top, x[j]);
+        }
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float m_new = fmaxf(m_run[n], top);
+        const float m_use = m_new == kNegInf ? 0.0f : m_new;
+        const float scale = exp2_fast(m_run[n] - m_use);
+        m_run[n] = m_new;
+        float sum = 0.0f;
+        u32x4 hw, lw;
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+          const float p0 = exp2_fast(x[j] - m_use), p1 = exp2_fast(x[j + 1] - m_use);
+          sum += p0 + p1;
+          // Weights in two 16-bit words (2^-16 of them left, 2^-22 in fp16): the
+          // second product costs nothing beside the cache's bytes.
+          hw[j >> 1] = E::pack(p0, p1);
+          lw[j >> 1] = E::pack(p0 - E::lo(hw[j >> 1]), p1 - E::hi(hw[j >> 1]));
+        }
+        hi[n] = __builtin_bit_cast(vec_t, hw);
+        lo[n] = __builtin_bit_cast(vec_t, lw);
+        l_run[n] = l_run[n] * scale + sum;
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) acc[n][b] *= scale;
+      }
+
+      // The wave reads what it wrote itself: its LDS operations keep their order.
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) {
+        const int row = 4 * group + (col >> 2), c = 2 * b + ((col & 3) >> 1), half = 4 * (col & 1);
+        const s16x4 v0 = read_column(&v_stage[wave][Layout::at(row, c) + half]);
+        const s16x4 v1 = read_column(&v_stage[wave][Layout::at(row + 16, c) + half]);
+        vec_t vf = join_columns<vec_t>(v0, v1);
+        if (careful) {
+          // Values that are not finite are added only to the rows that see them,
+          // token by token, by the first word of their weights.
+          s16x8 raw = __builtin_bit_cast(s16x8, vf), odd = {0, 0, 0, 0, 0, 0, 0, 0};
+          bool any = false;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if ((static_cast<uint16_t>(raw[j]) & E::kExponent) == E::kExponent) {
+              odd[j] = raw[j];
+              raw[j] = 0;
+              any = true;
+            }
+          vf = __builtin_bit_cast(vec_t, raw);
+          if (__any(any)) {
+            for (int i = 0; i < s.fresh; ++i) {
+              const RowSight one = sight_of(a, s, place0 + i);
+              s16x8 seen = odd;
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (!sees(one, a.sinks, key0 + 16 * (j >> 2) + 4 * group + (j & 3))) seen[j] = 0;
+#pragma unroll
+              for (int n = 0; n < NQ; ++n) {
+                const f32x4 more = E::mfma(__builtin_bit_cast(vec_t, seen), hi[n], f32x4{0, 0, 0, 0});
+                if ((n * 16 + col) / a.qpk == i) acc[n][b] += more;
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+          acc[n][b] = E::mfma(vf, hi[n], acc[n][b]);
+          acc[n][b] = E::mfma(vf, lo[n], acc[n][b]);
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+    bool wild = false;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) wild |= !(fabsf(acc[n][b][i]) <= 3.4e38f);
+    if (careful || !__any(wild)) break;
+    }
+
+    // Join the four waves: a common maximum, then sums.
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      float l = l_run[n];
+      l += __shfl_xor(l, 16);
+      l += __shfl_xor(l, 32);
+      l_run[n] = l;
+      if (group == 0) {
+        wave_m[wave][n * 16 + col] = m_run[n];
+        wave_l[wave][n * 16 + col] = l;
+      }
+    }
+    __syncthreads();
+    float m_all[NQ], l_all[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      const int m = n * 16 + col;
+      float top = kNegInf;
+#pragma unroll
+      for (int w = 0; w < kFewWaves; ++w) top = fmaxf(top, wave_m[w][m]);
+      const float use = top == kNegInf ? 0.0f : top;
+      float l = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kFewWaves; ++w) l += wave_l[w][m] * exp2_fast(wave_m[w][m] - use);
+      const float scale = exp2_fast(m_run[n] - use);
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) acc[n][b] *= scale;
+      m_all[n] = top;
+      l_all[n] = l;
+    }
+    // 16 rows x DP floats a tile and wave, waves 2, 3 then 1 into 0, 1 then 0.
+    float* const pool = reinterpret_cast<float*>(&v_stage[0][0]);
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+      for (int half = 2; half >= 1; half >>= 1) {
+        __syncthreads();
+        if (wave >= half && wave < 2 * half) {
+          float* to = pool + (wave - half) * (DP * 16);
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b) *reinterpret_cast<f32x4*>(to + (b * 64 + lane) * 4) = acc[n][b];
+        }
+        __syncthreads();
+        if (wave < half) {
+          const float* from = pool + wave * (DP * 16);
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b) acc[n][b] += *reinterpret_cast<const f32x4*>(from + (b * 64 + lane) * 4);
+        }
+      }
+
+    const bool complete = piece_first == 0 && piece_last == tiles;
+    if (wave == 0) {
+      const int kind = at == range_begin ? 0 : 1;
+      float* const piece = a.partial + (2 * static_cast<int64_t>(wg) + kind) * piece_floats(kRows, DP);
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        const int m = n * 16 + col;
+        if (m >= rows) continue;
+        if (complete) {
+          const float inv = l_all[n] == 0.0f ? 0.0f : 1.0f / l_all[n];
+          const int token = m / a.qpk, g = m - token * a.qpk;
+          uint16_t* to = a.out + (s.token0 + token) * a.out_token_stride + (head * a.qpk + g) * a.out_head_stride;
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b) {
+            const int d = b * 16 + group * 4;
+            if (d < a.head_dim)
+              *gptr(reinterpret_cast<u32x2*>(to + d)) = u32x2{E::pack(acc[n][b][0] * inv, acc[n][b][1] * inv), E::pack(acc[n][b][2] * inv, acc[n][b][3] * inv)};
+          }
+        } else {
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b) *gptr(reinterpret_cast<f32x4*>(piece + m * DP + b * 16 + group * 4)) = acc[n][b];
+          if (group == 0) *gptr(reinterpret_cast<f32x2*>(piece + kRows * DP + 2 * m)) = f32x2{m_all[n], l_all[n]};
+        }
+      }
+      if (!complete && piece_first == 0 && lane == 0) {
+        // The (request, head) goes on in the next workgroups: `count` pieces in all.
+        a.header[4 * wg] = r;
+        a.header[4 * wg + 1] = head;
+        a.header[4 * wg + 2] = (whole_begin + tiles - 1) / per - wg + 1;
+        a.header[4 * wg + 3] = kind;
+      }
+    }
+    at = piece_end;
+    __syncthreads();
+  }
+}
+
+// Joins the pieces of the (request, head) that begins in workgroup blockIdx.x
+// and ends in a later one: out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.
+template <bool F16, int DP, int NQ>
+__global__ __launch_bounds__(kFewThreads) void attend_few_join_kernel(AttendArgs a) {
+  typedef AttendElem<F16> E;
+  constexpr int kRows = 16 * NQ;
+  const int wg = blockIdx.x;
+  const int count = a.header[4 * wg + 2];
+  if (count < 2) return;
+  const int r = a.header[4 * wg], head = a.header[4 * wg + 1], kind = a.header[4 * wg + 3];
+  const Request s = request_of(a, r);
+  const int rows = s.fresh * a.qpk;
+  const int64_t size = piece_floats(kRows, DP);
+  const float* const first = a.partial + (2 * static_cast<int64_t>(wg) + kind) * size;
+  const float* const rest = a.partial + 2 * static_cast<int64_t>(wg) * size;  // piece i > 0 at 2*i*size
+  for (int u = threadIdx.x; u < rows * (DP / 4); u += kFewThreads) {
+    const int m = u / (DP / 4), d = (u - m * (DP / 4)) * 4;
+    if (d >= a.head_dim) continue;
+    float top = kNegInf;
+    for (int i = 0; i < count; ++i) top = fmaxf(top, (i ? rest + 2 * i * size : first)[kRows * DP + 2 * m]);
+    const float use = top == kNegInf ? 0.0f : top;
+    f32x4 sum = {0, 0, 0, 0};
+    float l = 0.0f;
+#pragma unroll 4
+    for (int i = 0; i < count; ++i) {
+      const float* p = i ? rest + 2 * i * size : first;
+      const f32x2 ml = *reinterpret_cast<const f32x2*>(p + kRows * DP + 2 * m);
+      const float w = exp2_fast(ml.x - use);
+      sum += *reinterpret_cast<const f32x4*>(p + m * DP + d) * w;
+      l += ml.y * w;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int token = m / a.qpk, g = m - token * a.qpk;
+    uint16_t* to = a.out + (s.token0 + token) * a.out_token_stride + (head * a.qpk + g) * a.out_head_stride;
+    *gptr(reinterpret_cast<u32x2*>(to + d)) = u32x2{E::pack(sum[0] * inv, sum[1] * inv), E::pack(sum[2] * inv, sum[3] * inv)};
+  }
+}
+
+template <bool F16, int DP, int NQ>
+int launch(hipStream_t stream, const AttendArgs& a, int workgroups) {
+  attend_few_kernel<F16, DP, NQ><<<workgroups, kFewThreads, 0, stream>>>(a);
+  if (int rc = launch_status("kvc_attend_paged")) return rc;
+  if (workgroups > 1) attend_few_join_kernel<F16, DP, NQ><<<workgroups, kFewThreads, 0, stream>>>(a);
+  return launch_status("kvc_attend_paged");
+}
+
+template <bool F16, int DP>
+int pick_rows(hipStream_t stream, const AttendArgs& a, int workgroups, int row_tiles) {
+  return row_tiles == 1 ? launch<F16, DP, 1>(stream, a, workgroups) : launch<F16, DP, 2>(stream, a, workgroups);
+}
+
+template <bool F16>
+int pick_dim(hipStream_t stream, const AttendArgs& a, int workgroups, int row_tiles) {
+  switch (padded_dim(a.head_dim)) {
+    case 64: return pick_rows<F16, 64>(stream, a, workgroups, row_tiles);
+    case 96: return pick_rows<F16, 96>(stream, a, workgroups, row_tiles);
+    case 128: return pick_rows<F16, 128>(stream, a, workgroups, row_tiles);
+    case 192: return pick_rows<F16, 192>(stream, a, workgroups, row_tiles);
+    default: return pick_rows<F16, 256>(stream, a, workgroups, row_tiles);
+  }
+}
+
+}  // namespace
+
+int launch_attend_few(hipStream_t stream, bool f16, const AttendArgs& a, int workgroups, int row_tiles) {
+  return f16 ? pick_dim<true>(stream, a, workgroups, row_tiles) : pick_dim<false>(stream, a, workgroups, row_tiles);
+}
+
+}  // namespace kvc

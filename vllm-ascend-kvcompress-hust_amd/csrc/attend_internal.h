@@ -1,0 +1,149 @@
+// Attention of new tokens over a paged cache: arguments, geometry and helpers
+// shared by the two kernels (attend_few.hip, attend_many.hip) and their entry
+// (attend.hip).
+//
+// For a request with `len` cached tokens (its new ones among them) and `fresh`
+// new tokens, token i sits at place p = len - fresh + i and sees the keys
+//   { j : j <= p  and  (window == 0 or p - j < window or j < sinks) },
+// and out = sum_j softmax_j(scale * q.k_j) v_j over them; a row that sees no
+// key gives zeros.  The query heads of one KV head are stacked: row
+// m = i*qpk + g is query head h*qpk + g of token i, so K and V are read once
+// for a whole group of heads.
+#pragma once
+
+#include "mfma_common.h"
+
+namespace kvc {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+#define KVC_LDS __attribute__((address_space(3)))
+
+struct AttendArgs {
+  const uint16_t* q;
+  uint16_t* out;
+  const uint16_t* k;
+  const uint16_t* v;
+  const int32_t* start;     // [n_seq + 1] first token of each request
+  const int32_t* seq_lens;  // [n_seq]
+  const int32_t* table;     // [n_seq][table_stride]
+  float* partial;           // joined pieces, see the kernels
+  int32_t* header;
+  int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+  int64_t num_pages, page_stride, table_stride, num_tokens;
+  float scale_log2;  // scale * log2(e): weights are powers of two
+  int n_seq, kv_heads, qpk, head_dim, max_blocks, window, sinks;
+  int few_rows;  // requests of at most this many rows are the few-rows kernel's
+};
+
+// One request's rows and keys.
+struct Request {
+  int token0, fresh;  // first token, new tokens
+  int len, keys;      // cached tokens; those that the block table covers
+};
+
+__device__ __forceinline__ Request request_of(const AttendArgs& a, int r) {
+  Request s;
+  const int64_t total = a.num_tokens;
+  int64_t t0 = a.start[r], t1 = a.start[r + 1];
+  t0 = t0 < 0 ? 0 : (t0 > total ? total : t0);
+  t1 = t1 < t0 ? t0 : (t1 > total ? total : t1);
+  s.token0 = static_cast<int>(t0);
+  s.fresh = static_cast<int>(t1 - t0);
+  const int len = a.seq_lens[r];
+  s.len = len < 0 ? 0 : len;
+  const int64_t most = static_cast<int64_t>(a.max_blocks) << kBlockShift;
+  s.keys = s.len < most ? s.len : static_cast<int>(most);
+  return s;
+}
+
+// Key tiles of 2^SHIFT keys that rows at places [first, last] see: the first
+// `head` ones (sinks that the window has left behind) and [low, high).
+struct TileRange {
+  int head, low, high;
+  __device__ __forceinline__ int count() const { return head + high - low; }
+  __device__ __forceinline__ int tile(int t) const { return t < head ? t : low + t - head; }
+};
+
+template <int SHIFT>
+__device__ __forceinline__ TileRange tile_range(const AttendArgs& a, const Request& s, int first, int last) {
+  TileRange p;
+  int end = last + 1 < s.keys ? last + 1 : s.keys;
+  if (end < 0) end = 0;
+  int begin = a.window ? first - a.window + 1 : 0;
+  begin = begin < 0 ? 0 : (begin > end ? end : begin);
+  p.low = begin >> SHIFT;
+  p.high = (end + (1 << SHIFT) - 1) >> SHIFT;
+  const int sink = a.sinks < begin ? a.sinks : begin;
+  p.head = (sink + (1 << SHIFT) - 1) >> SHIFT;
+  if (p.head > p.low) p.head = p.low;
+  return p;
+}
+
+// Keys that one row sees: [low, end) and those below `sinks` that are below end.
+struct RowSight {
+  int end, low;
+};
+
+__device__ __forceinline__ RowSight sight_of(const AttendArgs& a, const Request& s, int place) {
+  return {place + 1 < s.keys ? place + 1 : s.keys, a.window ? place - a.window + 1 : 0};
+}
+
+__device__ __forceinline__ bool sees(const RowSight& s, int sinks, int key) {
+  return key < s.end && (key >= s.low || key < sinks);
+}
+
+// The element type of a cache for the 32x32 products.
+template <bool F16>
+struct AttendElem : MfmaElem<F16> {
+  typedef typename MfmaElem<F16>::vec vec;
+  // Exponent bits: all set in infinities and NaN.
+  static constexpr uint32_t kExponent = F16 ? 0x7c00u : 0x7f80u;
+  __device__ __forceinline__ static f32x16 mfma32(vec a, vec b, f32x16 c) {
+    if constexpr (F16)
+      return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+
+// Four 16-bit values of one column: the 16 lanes of a group give the addresses
+// of four rows' 16 columns (lane k: row k/4, columns 4*(k%4)..), and lane k
+// gets column k of the four rows (ds_read_b64_tr_b16).
+__device__ __forceinline__ s16x4 read_column(const uint16_t* p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((KVC_LDS s16x4*)p);
+}
+
+template <typename V>
+__device__ __forceinline__ V join_columns(s16x4 a, s16x4 b) {
+  return __builtin_bit_cast(V, s16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+constexpr float kNegInf = -__builtin_inff();
+
+// Entry points of the kernels' files.
+int launch_attend_few(hipStream_t stream, bool f16, const AttendArgs& a, int workgroups, int row_tiles);
+int launch_attend_many(hipStream_t stream, bool f16, const AttendArgs& a, int64_t tiles, int splits);
+
+// Sizes of the workspace's parts.
+constexpr int kFewRows = 16;         // rows of one few-rows tile
+constexpr int kFewTilesMost = 2;     // tiles of a request that the few-rows kernel takes
+constexpr int kFewSequences = 2048;  // requests of one launch (their prefix sums sit in LDS)
+constexpr int kManyRows = 128;       // rows of one many-rows tile
+
+// Floats of a piece of `rows` rows: unnormalised outputs, then (max, sum) pairs.
+__host__ __device__ inline int64_t piece_floats(int rows, int dim) { return static_cast<int64_t>(rows) * (dim + 2); }
+
+// Head dims are computed in multiples of 32.
+inline int padded_dim(int head_dim) {
+  const int dims[] = {64, 96, 128, 192, 256};
+  for (int d : dims)
+    if (head_dim <= d) return d;
+  return 0;
+}
+
+}  // namespace kvc

@@ -1,0 +1,359 @@
+// Attention of requests with many rows (chunks of a prompt): the matrix cores
+// bound it.  A workgroup takes 128 rows of one (request, KV head), 32 a wave,
+// and walks the key tiles that some row sees; K and V tiles pass through LDS,
+// two buffers deep, the next tile's loads in registers while one is worked on.
+// With few tiles of rows the keys are split too, and a second launch joins the
+// splits.
+//
+// Scores are formed transposed (S^T = K Q^T, 32x32x16): a lane holds one row's
+// scores (its other half in lane ^ 32), so the softmax needs one exchange, and
+// the packed weights are the right operand of O^T = V^T P^T as they lie, keys
+// numbered to match: slot (lane/32, j) of 16 keys is key 8*(j/4) + 4*(lane/32)
+// + j%4.  Weights are rounded to the cache's 16-bit type for that product (the
+// error of a sum of them is that of one rounding, as the output's own is); the
+// maxima, sums and outputs stay in float32.
+
+#include "attend_internal.h"
+
+namespace kvc {
+namespace {
+
+constexpr int kManyThreads = 256;
+
+template <int DP>
+struct ManyLayout {
+  static constexpr int kKeys = DP <= 128 ? 64 : 32;
+  static constexpr int kShift = DP <= 128 ? 6 : 5;
+  static constexpr int kRow = DP <= 64 ? 64 : (DP <= 128 ? 128 : 256);  // LDS row, elements
+  static constexpr int kTile = kKeys * kRow;
+  // 16-byte chunks are moved so that the 16 rows of an operand read (K, one
+  // chunk of each) and the four rows of a column read (V, four chunks of each)
+  // fall on different banks.
+  __device__ __forceinline__ static int k_at(int row, int chunk) {
+    const int turn = kRow == 64 ? (row >> 1) & 7 : row & 15;
+    return row * kRow + ((chunk ^ turn) << 3);
+  }
+  __device__ __forceinline__ static int v_at(int row, int chunk) {
+    const int turn = kRow == 64 ? ((row >> 1) & 1) * 4 : (row & 3) * 4;
+    return row * kRow + ((chunk ^ turn) << 3);
+  }
+};
+
+// The row tile and request of a workgroup: request r owns tiles from
+// start[r]*qpk/128 + r, which leaves room for its last, partly filled one.
+struct ManyTile {
+  int request, row0;
+};
+
+__device__ __forceinline__ int64_t tile_base(const AttendArgs& a, int r) {
+  int64_t t = a.start[r];
+  t = t < 0 ? 0 : (t > a.num_tokens ? a.num_tokens : t);
+  return t * a.qpk / kManyRows + r;
+}
+
+__device__ __forceinline__ ManyTile tile_of(const AttendArgs& a, int64_t tile) {
+  int low = 0, high = a.n_seq;  // base(low) <= tile < base(high)
+  while (high - low > 1) {
+    const int mid = (low + high) >> 1;
+    if (tile_base(a, mid) <= tile)
+      low = mid;
+    else
+      high = mid;
+  }
+  const int64_t row0 = (tile - tile_base(a, low)) * kManyRows;
+  return {low, row0 < 0 || row0 > 0x7fffff00 ? 0x7fffff00 : static_cast<int>(row0)};
+}
+
+template <bool F16, int DP>
+__global__ __launch_bounds__(kManyThreads, DP <= 128 ? 2 : 1) void attend_many_kernel(AttendArgs a, int64_t tiles, int splits) {
+  typedef AttendElem<F16> E;
+  typedef typename E::vec vec_t;
+  typedef ManyLayout<DP> L;
+  constexpr int kSteps = DP / 16;       // 16-dim steps of K Q^T
+  constexpr int kBlocks = DP / 32;      // 32-dim blocks of the output
+  constexpr int kChunks = DP / 8;       // 16-byte chunks of a row
+  constexpr int kKeyBlocks = L::kKeys / 32;
+  constexpr int kLoads = L::kKeys * kChunks / kManyThreads;
+  __shared__ __attribute__((aligned(16))) uint16_t k_tile[2][L::kTile];
+  __shared__ __attribute__((aligned(16))) uint16_t v_tile[2][L::kTile];
+
+  const int head = blockIdx.x % a.kv_heads;
+  const int rest = blockIdx.x / a.kv_heads;
+  const int split = rest % splits;
+  const int64_t tile = tiles - 1 - rest / splits;  // the last rows see the most keys: they begin first
+  const ManyTile mine = tile_of(a, tile);
+  const Request s = request_of(a, mine.request);
+  const int64_t all_rows = static_cast<int64_t>(s.fresh) * a.qpk;
+  if (mine.row0 >= all_rows || all_rows <= a.few_rows) return;
+  const int rows = static_cast<int>(all_rows);
+
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 31, half = lane >> 5;
+  const int place0 = s.len - s.fresh;
+  const int wg_last = (mine.row0 + kManyRows < rows ? mine.row0 + kManyRows : rows) - 1;
+  const TileRange range = tile_range<L::kShift>(a, s, place0 + mine.row0 / a.qpk, place0 + wg_last / a.qpk);
+  const int count = range.count();
+  const int t_begin = static_cast<int>(static_cast<int64_t>(count) * split / splits);
+  const int t_end = static_cast<int>(static_cast<int64_t>(count) * (split + 1) / splits);
+
+  const int m = mine.row0 + wave * 32 + col;
+  const bool inside = m < rows;
+  const int token = (inside ? m : rows - 1) / a.qpk, g = (inside ? m : rows - 1) - token * a.qpk;
+  RowSight sight = sight_of(a, s, place0 + token);
+  if (!inside) sight.end = 0;
+  // The wave's first and last rows' sights.
+  const int m_first = mine.row0 + wave * 32, m_last = m_first + 31 < rows ? m_first + 31 : rows - 1;
+  const bool wave_rows = m_first < rows;
+  const int token_first = m_first / a.qpk, token_last = (wave_rows ? m_last : m_first) / a.qpk;
+  const RowSight first = sight_of(a, s, place0 + token_first), last = sight_of(a, s, place0 + token_last);
+
+  vec_t qf[kSteps];
+  {
+    const uint16_t* row = a.q + (s.token0 + token) * a.q_token_stride + (head * a.qpk + g) * a.q_head_stride;
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st) {
+      const int d = st * 16 + half * 8;
+      u32x4 w = {0, 0, 0, 0};
+      if (inside && d < a.head_dim) w = *gptr(reinterpret_cast<const u32x4*>(row + d));
+      qf[st] = __builtin_bit_cast(vec_t, w);
+    }
+  }
+  const int64_t row_elems = static_cast<int64_t>(a.kv_heads) * a.head_dim;
+  const int32_t* table = a.table + mine.request * a.table_stride;
+  u32x4 kst[kLoads], vst[kLoads];
+  bool next_valid = false;
+  auto load = [&](int t) {
+    const int key0 = range.tile(t) << L::kShift;
+    const int page = table[key0 >> kBlockShift];
+    next_valid = page >= 0 && page < a.num_pages;
+    if (!next_valid) return;
+    const int64_t base = page * a.page_stride + (key0 & (kBlockSize - 1)) * row_elems + head * a.head_dim;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int u = i * kManyThreads + tid, row = u / kChunks, c = u - row * kChunks;
+      kst[i] = u32x4{0, 0, 0, 0};
+      vst[i] = u32x4{0, 0, 0, 0};
+      if (c * 8 < a.head_dim) {
+        kst[i] = *gptr(reinterpret_cast<const u32x4*>(a.k + base + row * row_elems + c * 8));
+        vst[i] = *gptr(reinterpret_cast<const u32x4*>(a.v + base + row * row_elems + c * 8));
+      }
+    }
+  };
+
+  f32x16 acc[kBlocks];
+  float m_run, l_run;
+  // A weight of zero turns an infinity or NaN among V into NaN for rows that do
+  // not see it.  That shows in the outputs: a workgroup that finds one there
+  // goes over its keys again with care.
+  for (bool careful = false;; careful = true) {
+#pragma unroll
+  for (int b = 0; b < kBlocks; ++b) acc[b] = f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+  m_run = kNegInf;
+  l_run = 0.0f;
+  if (t_begin < t_end) load(t_begin);
+  for (int t = t_begin; t < t_end; ++t) {
+    uint16_t* const kt = k_tile[t & 1];
+    uint16_t* const vt = v_tile[t & 1];
+    const bool valid = next_valid;
+    const int key0 = range.tile(t) << L::kShift;
+    if (valid) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int u = i * kManyThreads + tid, row = u / kChunks, c = u - row * kChunks;
+        if (key0 + row >= s.keys) vst[i] = u32x4{0, 0, 0, 0};  // behind the request: whatever the page holds
+        *reinterpret_cast<u32x4*>(&kt[L::k_at(row, c)]) = kst[i];
+        *reinterpret_cast<u32x4*>(&vt[L::v_at(row, c)]) = vst[i];
+      }
+    }
+    // One barrier a tile: a wave past it has done with the other buffer, too.
+    __syncthreads();
+    if (t + 1 < t_end) load(t + 1);
+    if (!valid || !wave_rows) continue;
+    if (key0 >= last.end || (key0 + L::kKeys <= first.low && key0 >= a.sinks)) continue;
+    const bool whole = key0 + L::kKeys <= first.end && (key0 >= last.low || key0 + L::kKeys <= a.sinks);
+
+    f32x16 sc[kKeyBlocks];
+#pragma unroll
+    for (int kb = 0; kb < kKeyBlocks; ++kb) {
+      sc[kb] = f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+      for (int st = 0; st < kSteps; ++st) {
+        const vec_t kf = __builtin_bit_cast(vec_t, *reinterpret_cast<const u32x4*>(&kt[L::k_at(kb * 32 + col, 2 * st + half)]));
+        sc[kb] = E::mfma32(kf, qf[st], sc[kb]);
+      }
+    }
+    float top = kNegInf;
+#pragma unroll
+    for (int kb = 0; kb < kKeyBlocks; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        if (!whole && !sees(sight, a.sinks, key0 + kb * 32 + 8 * (i >> 2) + 4 * half + (i & 3))) sc[kb][i] = kNegInf;
+        top = fmaxf(top, sc[kb][i]);
+      }
+    top = fmaxf(top, __shfl_xor(top, 32)) * a.scale_log2;
+    // The maximum moves only when it grows by more than 2^8: weights then reach
+    // 2^8 at most, and most tiles leave the outputs unscaled.
+    const float m_new = top > m_run + 8.0f ? top : m_run;
+    if (__any(m_new != m_run)) {
+      const float scale = m_new == kNegInf ? 1.0f : exp2_fast(m_run - m_new);
+      l_run *= scale;
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) acc[b] *= scale;
+      m_run = m_new;
+    }
+    const float m_use = m_run == kNegInf ? 0.0f : m_run;
+    vec_t pf[kKeyBlocks][2];
+    float sum = 0.0f;
+#pragma unroll
+    for (int kb = 0; kb < kKeyBlocks; ++kb)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        u32x4 w;
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+          const float p0 = exp2_fast(fmaf(sc[kb][8 * h + j], a.scale_log2, -m_use));
+          const float p1 = exp2_fast(fmaf(sc[kb][8 * h + j + 1], a.scale_log2, -m_use));
+          sum += p0 + p1;
+          w[j >> 1] = E::pack(p0, p1);
+        }
+        pf[kb][h] = __builtin_bit_cast(vec_t, w);
+      }
+    l_run += sum;
+
+    const int v_row = 4 * half + ((lane & 15) >> 2);
+    const int v_chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), v_half = 4 * (lane & 1);
+#pragma unroll
+    for (int kb = 0; kb < kKeyBlocks; ++kb)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) {
+          const int row = kb * 32 + h * 16 + v_row, c = 4 * b + v_chunk;
+          const s16x4 v0 = read_column(&vt[L::v_at(row, c) + v_half]);
+          const s16x4 v1 = read_column(&vt[L::v_at(row + 8, c) + v_half]);
+          vec_t vf = join_columns<vec_t>(v0, v1);
+          if (careful) {
+            // Values that are not finite are added only to the rows that see
+            // them, token by token.
+            s16x8 raw = __builtin_bit_cast(s16x8, vf), odd = {0, 0, 0, 0, 0, 0, 0, 0};
+            bool any = false;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if ((static_cast<uint16_t>(raw[j]) & E::kExponent) == E::kExponent) {
+                odd[j] = raw[j];
+                raw[j] = 0;
+                any = true;
+              }
+            vf = __builtin_bit_cast(vec_t, raw);
+            if (__any(any)) {
+              for (int i = token_first; i <= token_last; ++i) {
+                const RowSight one = sight_of(a, s, place0 + i);
+                s16x8 seen = odd;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                  if (!sees(one, a.sinks, key0 + kb * 32 + h * 16 + 8 * (j >> 2) + 4 * half + (j & 3))) seen[j] = 0;
+                const f32x16 more =
+                    E::mfma32(__builtin_bit_cast(vec_t, seen), pf[kb][h], f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0});
+                if (token == i) acc[b] += more;
+              }
+            }
+          }
+          acc[b] = E::mfma32(vf, pf[kb][h], acc[b]);
+        }
+  }
+  bool wild = false;
+#pragma unroll
+  for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) wild |= !(fabsf(acc[b][i]) <= 3.4e38f);
+  if (careful || !__syncthreads_or(wild)) break;
+  }
+
+  const float l_all = l_run + __shfl_xor(l_run, 32);
+  if (!inside) return;
+  if (splits == 1) {
+    const float inv = l_all == 0.0f ? 0.0f : 1.0f / l_all;
+    uint16_t* to = a.out + (s.token0 + token) * a.out_token_stride + (head * a.qpk + g) * a.out_head_stride;
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = b * 32 + i * 8 + half * 4;
+        if (d < a.head_dim)
+          *gptr(reinterpret_cast<u32x2*>(to + d)) =
+              u32x2{E::pack(acc[b][4 * i] * inv, acc[b][4 * i + 1] * inv), E::pack(acc[b][4 * i + 2] * inv, acc[b][4 * i + 3] * inv)};
+      }
+  } else {
+    float* const piece = a.partial + ((tile * a.kv_heads + head) * splits + split) * piece_floats(kManyRows, DP);
+    const int local = m - mine.row0;
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *gptr(reinterpret_cast<f32x4*>(piece + local * DP + b * 32 + i * 8 + half * 4)) =
+            f32x4{acc[b][4 * i], acc[b][4 * i + 1], acc[b][4 * i + 2], acc[b][4 * i + 3]};
+    if (half == 0) *gptr(reinterpret_cast<f32x2*>(piece + kManyRows * DP + 2 * local)) = f32x2{m_run, l_all};
+  }
+}
+
+// Joins the splits of a (row tile, KV head).
+template <bool F16, int DP>
+__global__ __launch_bounds__(kManyThreads) void attend_many_join_kernel(AttendArgs a, int splits) {
+  typedef AttendElem<F16> E;
+  const int head = blockIdx.x % a.kv_heads;
+  const int64_t tile = blockIdx.x / a.kv_heads;
+  const ManyTile mine = tile_of(a, tile);
+  const Request s = request_of(a, mine.request);
+  const int64_t all_rows = static_cast<int64_t>(s.fresh) * a.qpk;
+  if (mine.row0 >= all_rows || all_rows <= a.few_rows) return;
+  const int rows = all_rows - mine.row0 < kManyRows ? static_cast<int>(all_rows - mine.row0) : kManyRows;
+  const int64_t size = piece_floats(kManyRows, DP);
+  const float* const pieces = a.partial + (tile * a.kv_heads + head) * splits * size;
+  for (int u = threadIdx.x; u < rows * (DP / 4); u += kManyThreads) {
+    const int local = u / (DP / 4), d = (u - local * (DP / 4)) * 4;
+    if (d >= a.head_dim) continue;
+    float top = kNegInf;
+    for (int i = 0; i < splits; ++i) top = fmaxf(top, pieces[i * size + kManyRows * DP + 2 * local]);
+    const float use = top == kNegInf ? 0.0f : top;
+    f32x4 sum = {0, 0, 0, 0};
+    float l = 0.0f;
+    for (int i = 0; i < splits; ++i) {
+      const f32x2 ml = *reinterpret_cast<const f32x2*>(pieces + i * size + kManyRows * DP + 2 * local);
+      const float w = exp2_fast(ml.x - use);
+      sum += *reinterpret_cast<const f32x4*>(pieces + i * size + local * DP + d) * w;
+      l += ml.y * w;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int m = mine.row0 + local, token = m / a.qpk, g = m - token * a.qpk;
+    uint16_t* to = a.out + (s.token0 + token) * a.out_token_stride + (head * a.qpk + g) * a.out_head_stride;
+    *gptr(reinterpret_cast<u32x2*>(to + d)) = u32x2{E::pack(sum[0] * inv, sum[1] * inv), E::pack(sum[2] * inv, sum[3] * inv)};
+  }
+}
+
+template <bool F16, int DP>
+int launch(hipStream_t stream, const AttendArgs& a, int64_t tiles, int splits) {
+  attend_many_kernel<F16, DP>
+      <<<static_cast<unsigned>(tiles * a.kv_heads * splits), kManyThreads, 0, stream>>>(a, tiles, splits);
+  if (int rc = launch_status("kvc_attend_paged")) return rc;
+  if (splits > 1)
+    attend_many_join_kernel<F16, DP><<<static_cast<unsigned>(tiles * a.kv_heads), kManyThreads, 0, stream>>>(a, splits);
+  return launch_status("kvc_attend_paged");
+}
+
+template <bool F16>
+int pick_dim(hipStream_t stream, const AttendArgs& a, int64_t tiles, int splits) {
+  switch (padded_dim(a.head_dim)) {
+    case 64: return launch<F16, 64>(stream, a, tiles, splits);
+    case 96: return launch<F16, 96>(stream, a, tiles, splits);
+    case 128: return launch<F16, 128>(stream, a, tiles, splits);
+    case 192: return launch<F16, 192>(stream, a, tiles, splits);
+    default: return launch<F16, 256>(stream, a, tiles, splits);
+  }
+}
+
+}  // namespace
+
+int launch_attend_many(hipStream_t stream, bool f16, const AttendArgs& a, int64_t tiles, int splits) {
+  return f16 ? pick_dim<true>(stream, a, tiles, splits) : pick_dim<false>(stream, a, tiles, splits);
+}
+
+}  // namespace kvc

@@ -10,7 +10,8 @@
 // attention lengths shrink by the same offset (pkg/provider.py:707-728).
 //
 // All three are integer gathers over a few thousand entries per step: one
-// thread per entry, no LDS.
+// thread per entry, no LDS.  The step tables form all of them, and the block
+// table itself, from the requests' lengths in one launch.
 
 #include "kvc_common.h"
 
@@ -77,6 +78,82 @@ __global__ __launch_bounds__(kDecodeThreads) void shift_lengths_kernel(T* __rest
   seq_lens[r] = static_cast<T>(static_cast<int64_t>(seq_lens[r]) - offsets[r]);
 }
 
+struct StepTables {
+  const int32_t *computed, *fresh;
+  const int64_t *offsets, *ids, *id_offsets;
+  int32_t *start, *seq_lens, *table;
+  int64_t *positions, *slots;
+  int64_t table_stride, num_tokens;
+  int n_seq, expand, max_blocks, shares;
+};
+
+// Page j (of 128 tokens) of a request whose scheduler pages are ids[0 .. count),
+// each `expand` pages long; -1 where there is none.
+__device__ __forceinline__ int32_t step_page(const int64_t* ids, int64_t count, int expand, int j) {
+  const int at = j / expand;
+  if (at >= count) return -1;
+  const int64_t id = ids[at];
+  if (id < 0 || id > (0x7fffffffll - expand) / expand) return -1;
+  return static_cast<int32_t>(id) * expand + (j - at * expand);
+}
+
+// Workgroup (r, share) writes request r's row of every table, the row's entries
+// and tokens spread over the shares; the workgroups behind the last request
+// write the padding tokens.  Each adds up the new tokens before its request
+// itself (a request's count is 4 bytes): no launch or wait between the sum and
+// its readers.
+__global__ __launch_bounds__(kDecodeThreads) void step_tables_kernel(StepTables a) {
+  __shared__ int64_t part[kDecodeThreads / 64];
+  const int r = blockIdx.x / a.shares, share = blockIdx.x - r * a.shares;
+  int64_t sum = 0;
+  for (int i = threadIdx.x; i < r; i += kDecodeThreads) {
+    const int n = a.fresh[i];
+    sum += n > 0 ? n : 0;
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  sum = 0;
+#pragma unroll
+  for (int w = 0; w < kDecodeThreads / 64; ++w) sum += part[w];
+  // Tokens that the buffers have no room for are dropped, here and for every request behind.
+  const int64_t start = sum < a.num_tokens ? sum : a.num_tokens;
+  const int thread = share * kDecodeThreads + threadIdx.x, threads = a.shares * kDecodeThreads;
+  if (r == a.n_seq) {
+    if (thread == 0) a.start[r] = static_cast<int32_t>(start);
+    for (int64_t i = start + thread; i < a.num_tokens; i += threads) {
+      a.slots[i] = -1;
+      a.positions[i] = 0;
+    }
+    return;
+  }
+  const int64_t wanted = a.fresh[r] > 0 ? a.fresh[r] : 0;
+  const int64_t fresh = wanted < a.num_tokens - start ? wanted : a.num_tokens - start;
+  const int64_t computed = a.computed[r], offset = a.offsets ? a.offsets[r] : 0;
+  int64_t len = computed + fresh - offset;
+  len = len < 0 ? 0 : (len > 0x7fffffff ? 0x7fffffff : len);
+  if (thread == 0) {
+    a.start[r] = static_cast<int32_t>(start);
+    a.seq_lens[r] = static_cast<int32_t>(len);
+  }
+  const int64_t first = a.id_offsets[r], count = a.id_offsets[r + 1] - first;
+  const int64_t* ids = a.ids + first;
+  for (int j = thread; j < a.max_blocks; j += threads)
+    a.table[r * a.table_stride + j] =
+        static_cast<int64_t>(j) << kBlockShift < len ? step_page(ids, count, a.expand, j) : -1;
+  for (int64_t i = thread; i < fresh; i += threads) {
+    const int64_t p = computed + i - offset, j = p >> kBlockShift;
+    int64_t slot = -1;
+    if (p >= 0 && j < a.max_blocks) {
+      const int64_t page = step_page(ids, count, a.expand, static_cast<int>(j));
+      if (page >= 0) slot = (page << kBlockShift) + (p & (kBlockSize - 1));
+    }
+    a.slots[start + i] = slot;
+    a.positions[start + i] = computed + i;
+  }
+}
+
 }  // namespace
 }  // namespace kvc
 
@@ -130,4 +207,31 @@ extern "C" int kvc_shift_lengths(kvc_stream_t stream, void* seq_lens, int elem_b
     shift_lengths_kernel<int64_t><<<blocks, kDecodeThreads, 0, as_stream(stream)>>>(static_cast<int64_t*>(seq_lens),
                                                                                      request_offsets, num_reqs);
   return launch_status("kvc_shift_lengths");
+}
+
+extern "C" int kvc_step_tables(kvc_stream_t stream, int n_seq, const int32_t* computed_tokens, const int32_t* new_tokens,
+                               const int64_t* request_offsets, const int64_t* block_ids, const int64_t* block_offsets,
+                               int page_tokens, int max_query_len, int64_t num_tokens, int max_blocks, int64_t block_table_stride,
+                               int32_t* query_start_loc, int32_t* seq_lens, int64_t* positions, int64_t* slot_mapping,
+                               int32_t* block_table) {
+  if (n_seq < 0 || n_seq >= (1 << 24) || num_tokens < 0 || num_tokens >= (1ll << 31) || max_query_len < 0)
+    return fail(KVC_EINVAL, "kvc_step_tables: bad sizes");
+  if (page_tokens <= 0 || page_tokens % kBlockSize)
+    return fail(KVC_EINVAL, "kvc_step_tables: page_tokens must be a positive multiple of %d", kBlockSize);
+  if (max_blocks < 0 || max_blocks >= (1 << 24) || block_table_stride < max_blocks)
+    return fail(KVC_EINVAL, "kvc_step_tables: max_blocks must be below 2^24 and at most block_table_stride");
+  if (!query_start_loc || (num_tokens > 0 && (!positions || !slot_mapping)) ||
+      (n_seq > 0 && (!computed_tokens || !new_tokens || !block_offsets || !seq_lens || (max_blocks > 0 && !block_table))))
+    return fail(KVC_EINVAL, "kvc_step_tables: null pointer");
+  // About four entries or tokens a thread, as far as the device has room for workgroups.
+  const int64_t most = max_query_len > max_blocks ? max_query_len : max_blocks;
+  int64_t shares = ceil_div(most, 4 * kDecodeThreads);
+  const int64_t room = ceil_div(4096, n_seq + 1);
+  if (shares > room) shares = room;
+  if (shares < 1) shares = 1;
+  StepTables a = {computed_tokens, new_tokens, request_offsets, block_ids, block_offsets, query_start_loc, seq_lens, block_table,
+                  positions, slot_mapping, block_table_stride, num_tokens, n_seq, page_tokens / kBlockSize, max_blocks,
+                  static_cast<int>(shares)};
+  step_tables_kernel<<<static_cast<unsigned>((n_seq + 1) * shares), kDecodeThreads, 0, as_stream(stream)>>>(a);
+  return launch_status("kvc_step_tables");
 }

@@ -38,6 +38,7 @@ _i32 = ctypes.c_int
 _i64 = ctypes.c_int64
 _u32 = ctypes.c_uint
 _sz = ctypes.c_size_t
+_f32 = ctypes.c_float
 
 # name -> (restype, argtypes); the order of declaration follows the header.
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
@@ -103,6 +104,22 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "kvc_shift_positions": (_i32, [_p, _p, _p, _i32, _p, _i64, _p]),
     "kvc_physical_slot_mapping": (_i32, [_p, _i32, _p, _p, _p, _p, _i64, _i32, _i32, _i64, _p, _p]),
     "kvc_shift_lengths": (_i32, [_p, _p, _i32, _p, _i32]),
+    "kvc_step_tables": (_i32, [_p, _i32, _p, _p, _p, _p, _p, _i32, _i32, _i64, _i32, _i64, _p, _p, _p, _p, _p]),
+    "kvc_rotate_and_store": (
+        _i32,
+        [
+            _p, _i32, _i32, _i64, _i32, _i32, _i32, _i32, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p,
+            _i64, _i32, _p, _i32, _p, _p, _p, _i64, _i64, _p, _p, _i64, _i64,
+        ],
+    ),
+    "kvc_attend_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i64, _i32, _i32]),
+    "kvc_attend_paged": (
+        _i32,
+        [
+            _p, _i32, _p, _i64, _i64, _p, _p, _i64, _i64, _i32, _i32, _i32, _i32, _i64, _p, _p, _p, _i64, _i32,
+            _i32, _i32, _f32, _i32, _i32, _p, _i64, _i64, _p, _sz,
+        ],
+    ),
     "kvc_qstats_state_bytes": (_sz, [_i32, _i32, _i32]),
     "kvc_qstats_accumulate": (_i32, [_p, _i32, _p, _i64, _i64, _i32, _i32, _i32, _p, _sz]),
     "kvc_qstats_start": (_i32, [_p, _i32, _p, _i64, _i64, _i32, _i32, _i32, _p, _sz]),

@@ -7,6 +7,7 @@ from collections import OrderedDict
 import torch
 
 from ... import _native
+from ...config import KERNEL_BLOCK_SIZE as BLOCK_SIZE
 
 
 def require_hip(tensor: torch.Tensor, name: str) -> None:
