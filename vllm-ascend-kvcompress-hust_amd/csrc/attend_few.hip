@@ -23,15 +23,21 @@ constexpr int kFewThreads = 256;
 constexpr int kFewWaves = 4;
 constexpr int kSliceKeys = 32;  // keys of a wave's slice of a page
 
-// LDS row length of V (a power of two of 16-byte chunks) and the place of a
-// chunk: the 32-byte pairs of eight rows' same columns fall on different banks.
+// V's place in LDS: rows of 64, 128 or 256 elements, whose 32-byte pairs are
+// moved (an exclusive or with the row's `turn`) so that eight rows' same columns
+// fall on different banks.  Lane l holds, of every kStep rows, row l / kSlots and
+// 16-byte chunk l % kSlots.
 template <int DP>
 struct FewLayout {
   static constexpr int kRow = DP <= 64 ? 64 : (DP <= 128 ? 128 : 256);
-  __device__ __forceinline__ static int at(int row, int chunk) {
-    const int turn = kRow == 64 ? (row >> 1) & 3 : row & 7;
-    return row * kRow + ((chunk ^ (2 * turn)) << 3);
-  }
+  static constexpr int kSlots = kRow / 8;
+  static constexpr int kStep = 64 / kSlots;
+  static constexpr int kLoads = kSliceKeys / kStep;
+  static constexpr int kBytes = kSliceKeys * kRow * 2;
+  __device__ __forceinline__ static constexpr int turn(int row) { return kRow == 64 ? (row >> 1) & 3 : row & 7; }
+  // Byte place of the lane's chunk of load i: `to` is that of load 0, whose rows
+  // are below kStep, so the other rows' turns only set further bits.
+  __device__ __forceinline__ static int chunk_at(int to, int i) { return (to ^ (turn(i * kStep) << 5)) + i * kStep * kRow * 2; }
 };
 
 // Waves a SIMD: as many as the registers of a variant's outputs, queries and
@@ -44,8 +50,6 @@ __global__ __launch_bounds__(kFewThreads, few_waves(DP, NQ)) void attend_few_ker
   typedef typename E::vec vec_t;
   constexpr int kSteps = DP / 32;   // 32-dim steps of K Q^T
   constexpr int kBlocks = DP / 16;  // 16-dim blocks of the output
-  constexpr int kChunks = DP / 8;   // 16-byte chunks of a row
-  constexpr int kLoads = kSliceKeys * kChunks / 64;
   constexpr int kRows = 16 * NQ;
   typedef FewLayout<DP> Layout;
   __shared__ __attribute__((aligned(16))) uint16_t v_stage[kFewWaves][kSliceKeys * Layout::kRow];
@@ -53,7 +57,8 @@ __global__ __launch_bounds__(kFewThreads, few_waves(DP, NQ)) void attend_few_ker
   __shared__ float wave_m[kFewWaves][kRows], wave_l[kFewWaves][kRows];
   __shared__ int wave_sum[kFewWaves];
 
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, group = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, group = lane >> 4;
+  const int wave = uniform(tid >> 6);
 
   // Tiles before each request.
   if (tid == 0) before[0] = 0;
@@ -86,7 +91,7 @@ __global__ __launch_bounds__(kFewThreads, few_waves(DP, NQ)) void attend_few_ker
     carried += all;
     __syncthreads();
   }
-  const int total = before[a.n_seq];
+  const int total = uniform(before[a.n_seq]);
   const int per = (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
   const int wg = blockIdx.x;
   if (tid == 0) a.header[4 * wg + 2] = 0;  // no pieces to join until one begins here
@@ -97,18 +102,29 @@ __global__ __launch_bounds__(kFewThreads, few_waves(DP, NQ)) void attend_few_ker
 
   // The request that holds tile `at`.
   int r = 0;
-  for (int span = 1 << 10; span; span >>= 1)
+  for (int span = kFewSequences / 2; span; span >>= 1)
     if (r + span < a.n_seq && before[r + span] <= at) r += span;
 
-  const int64_t row_elems = static_cast<int64_t>(a.kv_heads) * a.head_dim;
+  const int row_elems = a.kv_heads * a.head_dim;
+  // The lane's places in a slice, in bytes: its K chunk of row `col`, its V chunk
+  // of the first rows (behind everything where the row has none), where that
+  // chunk goes, and the column it reads first.
+  const uint32_t row_bytes = row_elems * 2, k_lane = col * row_bytes + group * 16;
+  const int v_row = lane / Layout::kSlots, v_chunk = lane & (Layout::kSlots - 1), read_row = 4 * group + (col >> 2);
+  const uint32_t v_lane = v_chunk * 8 < a.head_dim ? v_row * row_bytes + v_chunk * 16 : 0x7fffffffu;
+  char* const stage = reinterpret_cast<char*>(&v_stage[wave][0]);
+  const int v_to = v_row * Layout::kRow * 2 + ((v_chunk * 16) ^ (Layout::turn(v_row) << 5));
+  const int v_from = read_row * Layout::kRow * 2 + (Layout::turn(read_row) << 5) + (col & 3) * 8;
   while (at < range_end) {
     while (before[r + 1] <= at) ++r;
+    r = uniform(r);
     const Request s = request_of(a, r);
     const TileRange pages = tile_range<kBlockShift>(a, s, s.len - s.fresh, s.len - 1);
-    const int tiles = (before[r + 1] - before[r]) / a.kv_heads;
-    const int head = (at - before[r]) / tiles;
-    const int piece_first = at - before[r] - head * tiles;
-    const int whole_begin = before[r] + head * tiles;
+    const int request_begin = uniform(before[r]);
+    const int tiles = (uniform(before[r + 1]) - request_begin) / a.kv_heads;
+    const int head = (at - request_begin) / tiles;
+    const int whole_begin = request_begin + head * tiles;
+    const int piece_first = at - whole_begin;
     const int piece_end = whole_begin + tiles < range_end ? whole_begin + tiles : range_end;
     const int piece_last = piece_end - whole_begin;
     const int rows = s.fresh * a.qpk;
@@ -140,6 +156,46 @@ __global__ __launch_bounds__(kFewThreads, few_waves(DP, NQ)) void attend_few_ker
     const int first_low = a.window ? place0 - a.window + 1 : 0;
     const int last_low = a.window ? s.len - a.window : 0;
 
+    // The next slice of this wave, from tile t on, that some row sees and whose
+    // page is in the pool.
+    struct Slice {
+      int tile, key0;
+      int64_t base;
+    };
+    const int32_t* const table = a.table + r * a.table_stride;
+    auto find = [&](int t) {
+      Slice f = {t, 0, 0};
+      if (pages.count() == 0) f.tile = piece_last;
+      for (; f.tile < piece_last; ++f.tile) {
+        const int block = pages.tile(f.tile);
+        f.key0 = (block << kBlockShift) + wave * kSliceKeys;
+        if (f.key0 >= last_end || (f.key0 + kSliceKeys <= first_low && f.key0 >= a.sinks)) continue;
+        const int page = uniform(table[block]);
+        if (page < 0 || page >= a.num_pages) continue;
+        f.base = page * a.page_stride + static_cast<int64_t>(wave * kSliceKeys) * row_elems + head * a.head_dim;
+        break;
+      }
+      return f;
+    };
+    // Buffer loads: a scalar base, 32-bit lane offsets, and zeros from behind the
+    // page (K) or the request's last row (V: whatever the page holds there).
+    u32x4 kw[2][kSteps], vw[Layout::kLoads];
+    auto load_k = [&](const Slice& f) {
+      const auto from = page_rsrc(a.k + f.base, kSliceKeys * row_bytes - head * a.head_dim * 2);
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int st = 0; st < kSteps; ++st)
+          kw[b][st] = __builtin_amdgcn_raw_buffer_load_b128(from, k_lane + st * 64, b * 16 * row_bytes, 0);
+    };
+    auto load_v = [&](const Slice& f) {
+      const int left = s.keys - f.key0 < kSliceKeys ? s.keys - f.key0 : kSliceKeys;
+      const auto from = page_rsrc(a.v + f.base, (left - 1) * row_bytes + a.head_dim * 2);
+#pragma unroll
+      for (int i = 0; i < Layout::kLoads; ++i)
+        vw[i] = __builtin_amdgcn_raw_buffer_load_b128(from, v_lane, i * Layout::kStep * row_bytes, 0);
+    };
+
     f32x4 acc[NQ][kBlocks];
     float m_run[NQ], l_run[NQ];
     // Weights of zero, and second words of any sign, turn an infinity or NaN
@@ -154,32 +210,21 @@ __global__ __launch_bounds__(kFewThreads, few_waves(DP, NQ)) void attend_few_ker
       for (int b = 0; b < kBlocks; ++b) acc[n][b] = f32x4{0, 0, 0, 0};
     }
 
-    for (int t = piece_first; t < piece_last; ++t) {
-      if (pages.count() == 0) break;
-      const int block = pages.tile(t);
-      const int page = a.table[r * a.table_stride + block];
-      if (page < 0 || page >= a.num_pages) continue;  // nothing of it is seen
-      const int key0 = (block << kBlockShift) + wave * kSliceKeys;
-      if (key0 >= last_end || (key0 + kSliceKeys <= first_low && key0 >= a.sinks)) continue;
+    Slice now = find(piece_first);
+    if (now.tile < piece_last) {
+      load_k(now);
+      load_v(now);
+    }
+    while (now.tile < piece_last) {
+      const int key0 = now.key0;
       const bool whole = key0 + kSliceKeys <= first_end && (key0 >= last_low || key0 + kSliceKeys <= a.sinks);
-      const int64_t base = page * a.page_stride + (wave * kSliceKeys) * row_elems + head * a.head_dim;
-      const uint16_t* kp = a.k + base;
-      const uint16_t* vp = a.v + base;
-
-      u32x4 kw[2][kSteps], vw[kLoads];
+      const Slice next = find(now.tile + 1);
+      if (a.head_dim != DP) {
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int st = 0; st < kSteps; ++st) {
-          const int d = st * 32 + group * 8;
-          kw[b][st] = u32x4{0, 0, 0, 0};
-          if (d < a.head_dim) kw[b][st] = *gptr(reinterpret_cast<const u32x4*>(kp + (b * 16 + col) * row_elems + d));
-        }
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int u = i * 64 + lane, row = u / kChunks, c = u - row * kChunks;
-        vw[i] = u32x4{0, 0, 0, 0};
-        if (c * 8 < a.head_dim) vw[i] = *gptr(reinterpret_cast<const u32x4*>(vp + row * row_elems + c * 8));
+          for (int st = 0; st < kSteps; ++st)
+            if (st * 32 + group * 8 >= a.head_dim) kw[b][st] = u32x4{0, 0, 0, 0};
       }
 
       f32x4 sc[NQ][2];
@@ -191,12 +236,7 @@ __global__ __launch_bounds__(kFewThreads, few_waves(DP, NQ)) void attend_few_ker
 #pragma unroll
           for (int st = 0; st < kSteps; ++st) sc[n][b] = E::mfma(__builtin_bit_cast(vec_t, kw[b][st]), qf[n][st], sc[n][b]);
         }
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int u = i * 64 + lane, row = u / kChunks, c = u - row * kChunks;
-        if (key0 + row >= s.keys) vw[i] = u32x4{0, 0, 0, 0};  // behind the request: whatever the page holds
-        *reinterpret_cast<u32x4*>(&v_stage[wave][Layout::at(row, c)]) = vw[i];
-      }
+      if (next.tile < piece_last) load_k(next);
 
       vec_t hi[NQ], lo[NQ];
 #pragma unroll
@@ -232,13 +272,16 @@ __global__ __launch_bounds__(kFewThreads, few_waves(DP, NQ)) void attend_few_ker
         for (int b = 0; b < kBlocks; ++b) acc[n][b] *= scale;
       }
 
+#pragma unroll
+      for (int i = 0; i < Layout::kLoads; ++i) *reinterpret_cast<u32x4*>(stage + Layout::chunk_at(v_to, i)) = vw[i];
+      if (next.tile < piece_last) load_v(next);
       // The wave reads what it wrote itself: its LDS operations keep their order.
       __builtin_amdgcn_wave_barrier();
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b) {
-        const int row = 4 * group + (col >> 2), c = 2 * b + ((col & 3) >> 1), half = 4 * (col & 1);
-        const s16x4 v0 = read_column(&v_stage[wave][Layout::at(row, c) + half]);
-        const s16x4 v1 = read_column(&v_stage[wave][Layout::at(row + 16, c) + half]);
+        const char* from = stage + (v_from ^ ((b & 7) << 5)) + (b >> 3) * 256;
+        const s16x4 v0 = read_column(from);
+        const s16x4 v1 = read_column(from + 16 * Layout::kRow * 2);
         vec_t vf = join_columns<vec_t>(v0, v1);
         if (careful) {
           // Values that are not finite are added only to the rows that see them,
@@ -275,6 +318,7 @@ __global__ __launch_bounds__(kFewThreads, few_waves(DP, NQ)) void attend_few_ker
         }
       }
       __builtin_amdgcn_wave_barrier();
+      now = next;
     }
     bool wild = false;
 #pragma unroll

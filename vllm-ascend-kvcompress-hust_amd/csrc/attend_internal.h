@@ -112,13 +112,21 @@ struct AttendElem : MfmaElem<F16> {
 // Four 16-bit values of one column: the 16 lanes of a group give the addresses
 // of four rows' 16 columns (lane k: row k/4, columns 4*(k%4)..), and lane k
 // gets column k of the four rows (ds_read_b64_tr_b16).
-__device__ __forceinline__ s16x4 read_column(const uint16_t* p) {
+__device__ __forceinline__ s16x4 read_column(const void* p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((KVC_LDS s16x4*)p);
 }
 
 template <typename V>
 __device__ __forceinline__ V join_columns(s16x4 a, s16x4 b) {
   return __builtin_bit_cast(V, s16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
+}
+
+// A value that every lane holds alike, as a scalar.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// A buffer of `bytes` bytes for loads with lane offsets; past its end they give zeros.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t page_rsrc(const uint16_t* base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, bytes, 0x00020000);
 }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -132,7 +140,7 @@ int launch_attend_many(hipStream_t stream, bool f16, const AttendArgs& a, int64_
 // Sizes of the workspace's parts.
 constexpr int kFewRows = 16;         // rows of one few-rows tile
 constexpr int kFewTilesMost = 2;     // tiles of a request that the few-rows kernel takes
-constexpr int kFewSequences = 2048;  // requests of one launch (their prefix sums sit in LDS)
+constexpr int kFewSequences = 1024;  // requests of one launch (their prefix sums sit in LDS)
 constexpr int kManyRows = 128;       // rows of one many-rows tile
 
 // Floats of a piece of `rows` rows: unnormalised outputs, then (max, sum) pairs.

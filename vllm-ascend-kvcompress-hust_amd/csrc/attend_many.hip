@@ -20,23 +20,23 @@ namespace {
 
 constexpr int kManyThreads = 256;
 
+// K's and V's place in LDS: rows of 64, 128 or 256 elements whose 16-byte chunks
+// are moved, by an exclusive or with a number of the row, so that the 16 rows of
+// an operand read (K, one chunk of each) and the four rows of a column read (V,
+// four chunks of each) fall on different banks.  A thread holds, of every kStep
+// rows, row tid / kSlots and chunk tid % kSlots.
 template <int DP>
 struct ManyLayout {
   static constexpr int kKeys = DP <= 128 ? 64 : 32;
   static constexpr int kShift = DP <= 128 ? 6 : 5;
-  static constexpr int kRow = DP <= 64 ? 64 : (DP <= 128 ? 128 : 256);  // LDS row, elements
+  static constexpr int kRow = DP <= 64 ? 64 : (DP <= 128 ? 128 : 256);
+  static constexpr int kBytes = kRow * 2;
   static constexpr int kTile = kKeys * kRow;
-  // 16-byte chunks are moved so that the 16 rows of an operand read (K, one
-  // chunk of each) and the four rows of a column read (V, four chunks of each)
-  // fall on different banks.
-  __device__ __forceinline__ static int k_at(int row, int chunk) {
-    const int turn = kRow == 64 ? (row >> 1) & 7 : row & 15;
-    return row * kRow + ((chunk ^ turn) << 3);
-  }
-  __device__ __forceinline__ static int v_at(int row, int chunk) {
-    const int turn = kRow == 64 ? ((row >> 1) & 1) * 4 : (row & 3) * 4;
-    return row * kRow + ((chunk ^ turn) << 3);
-  }
+  static constexpr int kSlots = kRow / 8;
+  static constexpr int kStep = kManyThreads / kSlots;
+  static constexpr int kLoads = kKeys / kStep;
+  __device__ __forceinline__ static constexpr int k_turn(int row) { return (kRow == 64 ? (row >> 1) & 7 : row & 15) << 4; }
+  __device__ __forceinline__ static constexpr int v_turn(int row) { return (kRow == 64 ? (row >> 1) & 1 : row & 3) << 6; }
 };
 
 // The row tile and request of a workgroup: request r owns tiles from
@@ -71,9 +71,7 @@ __global__ __launch_bounds__(kManyThreads, DP <= 128 ? 2 : 1) void attend_many_k
   typedef ManyLayout<DP> L;
   constexpr int kSteps = DP / 16;       // 16-dim steps of K Q^T
   constexpr int kBlocks = DP / 32;      // 32-dim blocks of the output
-  constexpr int kChunks = DP / 8;       // 16-byte chunks of a row
   constexpr int kKeyBlocks = L::kKeys / 32;
-  constexpr int kLoads = L::kKeys * kChunks / kManyThreads;
   __shared__ __attribute__((aligned(16))) uint16_t k_tile[2][L::kTile];
   __shared__ __attribute__((aligned(16))) uint16_t v_tile[2][L::kTile];
 
@@ -87,7 +85,8 @@ __global__ __launch_bounds__(kManyThreads, DP <= 128 ? 2 : 1) void attend_many_k
   if (mine.row0 >= all_rows || all_rows <= a.few_rows) return;
   const int rows = static_cast<int>(all_rows);
 
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 31, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
+  const int wave = uniform(tid >> 6);
   const int place0 = s.len - s.fresh;
   const int wg_last = (mine.row0 + kManyRows < rows ? mine.row0 + kManyRows : rows) - 1;
   const TileRange range = tile_range<L::kShift>(a, s, place0 + mine.row0 / a.qpk, place0 + wg_last / a.qpk);
@@ -117,26 +116,34 @@ __global__ __launch_bounds__(kManyThreads, DP <= 128 ? 2 : 1) void attend_many_k
       qf[st] = __builtin_bit_cast(vec_t, w);
     }
   }
-  const int64_t row_elems = static_cast<int64_t>(a.kv_heads) * a.head_dim;
+  const int row_elems = a.kv_heads * a.head_dim;
+  const uint32_t row_bytes = row_elems * 2;
   const int32_t* table = a.table + mine.request * a.table_stride;
-  u32x4 kst[kLoads], vst[kLoads];
+  // The thread's chunk of a tile's first rows: where it is (behind everything
+  // where the row has none) and where it goes, then where the lane reads.
+  const int row_to = tid / L::kSlots, chunk_to = tid & (L::kSlots - 1);
+  const uint32_t from = chunk_to * 8 < a.head_dim ? row_to * row_bytes + chunk_to * 16 : 0x7fffffffu;
+  const int k_to = row_to * L::kBytes + ((chunk_to << 4) ^ L::k_turn(row_to));
+  const int v_to = row_to * L::kBytes + ((chunk_to << 4) ^ L::v_turn(row_to));
+  const int k_from = col * L::kBytes + ((half << 4) ^ L::k_turn(col));
+  const int v_row = 4 * half + ((lane & 15) >> 2);
+  const int v_from = v_row * L::kBytes + L::v_turn(v_row) + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+  u32x4 kst[L::kLoads], vst[L::kLoads];
   bool next_valid = false;
   auto load = [&](int t) {
     const int key0 = range.tile(t) << L::kShift;
-    const int page = table[key0 >> kBlockShift];
+    const int page = uniform(table[key0 >> kBlockShift]);
     next_valid = page >= 0 && page < a.num_pages;
     if (!next_valid) return;
-    const int64_t base = page * a.page_stride + (key0 & (kBlockSize - 1)) * row_elems + head * a.head_dim;
+    const int64_t base = page * a.page_stride + static_cast<int64_t>(key0 & (kBlockSize - 1)) * row_elems + head * a.head_dim;
+    // Zeros from behind the request's last row, whatever the page holds there.
+    const int left = s.keys - key0 < L::kKeys ? s.keys - key0 : L::kKeys;
+    const uint32_t bytes = (left - 1) * row_bytes + a.head_dim * 2;
+    const auto k_page = page_rsrc(a.k + base, bytes), v_page = page_rsrc(a.v + base, bytes);
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int u = i * kManyThreads + tid, row = u / kChunks, c = u - row * kChunks;
-      kst[i] = u32x4{0, 0, 0, 0};
-      vst[i] = u32x4{0, 0, 0, 0};
-      if (c * 8 < a.head_dim) {
-        kst[i] = *gptr(reinterpret_cast<const u32x4*>(a.k + base + row * row_elems + c * 8));
-        vst[i] = *gptr(reinterpret_cast<const u32x4*>(a.v + base + row * row_elems + c * 8));
-      }
-    }
+    for (int i = 0; i < L::kLoads; ++i) kst[i] = __builtin_amdgcn_raw_buffer_load_b128(k_page, from, i * L::kStep * row_bytes, 0);
+#pragma unroll
+    for (int i = 0; i < L::kLoads; ++i) vst[i] = __builtin_amdgcn_raw_buffer_load_b128(v_page, from, i * L::kStep * row_bytes, 0);
   };
 
   f32x16 acc[kBlocks];
@@ -151,17 +158,15 @@ __global__ __launch_bounds__(kManyThreads, DP <= 128 ? 2 : 1) void attend_many_k
   l_run = 0.0f;
   if (t_begin < t_end) load(t_begin);
   for (int t = t_begin; t < t_end; ++t) {
-    uint16_t* const kt = k_tile[t & 1];
-    uint16_t* const vt = v_tile[t & 1];
+    char* const kt = reinterpret_cast<char*>(k_tile[t & 1]);
+    char* const vt = reinterpret_cast<char*>(v_tile[t & 1]);
     const bool valid = next_valid;
     const int key0 = range.tile(t) << L::kShift;
     if (valid) {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int u = i * kManyThreads + tid, row = u / kChunks, c = u - row * kChunks;
-        if (key0 + row >= s.keys) vst[i] = u32x4{0, 0, 0, 0};  // behind the request: whatever the page holds
-        *reinterpret_cast<u32x4*>(&kt[L::k_at(row, c)]) = kst[i];
-        *reinterpret_cast<u32x4*>(&vt[L::v_at(row, c)]) = vst[i];
+      for (int i = 0; i < L::kLoads; ++i) {
+        *reinterpret_cast<u32x4*>(kt + (k_to ^ L::k_turn(i * L::kStep)) + i * L::kStep * L::kBytes) = kst[i];
+        *reinterpret_cast<u32x4*>(vt + v_to + i * L::kStep * L::kBytes) = vst[i];
       }
     }
     // One barrier a tile: a wave past it has done with the other buffer, too.
@@ -177,7 +182,8 @@ __global__ __launch_bounds__(kManyThreads, DP <= 128 ? 2 : 1) void attend_many_k
       sc[kb] = f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
       for (int st = 0; st < kSteps; ++st) {
-        const vec_t kf = __builtin_bit_cast(vec_t, *reinterpret_cast<const u32x4*>(&kt[L::k_at(kb * 32 + col, 2 * st + half)]));
+        const vec_t kf = __builtin_bit_cast(
+            vec_t, *reinterpret_cast<const u32x4*>(kt + (k_from ^ (st << 5)) + kb * 32 * L::kBytes));
         sc[kb] = E::mfma32(kf, qf[st], sc[kb]);
       }
     }
@@ -219,17 +225,15 @@ __global__ __launch_bounds__(kManyThreads, DP <= 128 ? 2 : 1) void attend_many_k
       }
     l_run += sum;
 
-    const int v_row = 4 * half + ((lane & 15) >> 2);
-    const int v_chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), v_half = 4 * (lane & 1);
 #pragma unroll
     for (int kb = 0; kb < kKeyBlocks; ++kb)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b) {
-          const int row = kb * 32 + h * 16 + v_row, c = 4 * b + v_chunk;
-          const s16x4 v0 = read_column(&vt[L::v_at(row, c) + v_half]);
-          const s16x4 v1 = read_column(&vt[L::v_at(row + 8, c) + v_half]);
+          const char* at = vt + (v_from ^ (b << 6)) + (kb * 32 + h * 16) * L::kBytes;
+          const s16x4 v0 = read_column(at);
+          const s16x4 v1 = read_column(at + 8 * L::kBytes);
           vec_t vf = join_columns<vec_t>(v0, v1);
           if (careful) {
             // Values that are not finite are added only to the rows that see

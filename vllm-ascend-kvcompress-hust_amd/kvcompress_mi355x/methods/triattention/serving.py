@@ -29,15 +29,17 @@ from ... import _native
 from . import _device as dev
 
 AXIS_ORDERS = ("blocked", "cycled")
+_DTYPE_CODES = {torch.bfloat16: _native.DTYPE_BF16, torch.float16: _native.DTYPE_FP16}
 
 
-def _same_device(device: torch.device, **tensors: torch.Tensor | None) -> None:
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        dev.require_hip(t, name)
-        if t.device != device:
-            raise ValueError(f"{name} is on {t.device}, the step's other tensors are on {device}")
+# A small step's launches take a few microseconds each, so the checks below ask
+# each tensor little and look closer only to name what is wrong.
+
+
+def _misplaced(tensor: torch.Tensor, name: str, like: torch.Tensor) -> ValueError:
+    dev.require_hip(like, "the step's tensors")
+    dev.require_hip(tensor, name)
+    return ValueError(f"{name} is on {tensor.device}, the step's other tensors are on {like.device}")
 
 
 def _call(device: torch.device, name: str, *args: object) -> None:
@@ -49,12 +51,36 @@ def _call(device: torch.device, name: str, *args: object) -> None:
             _native.call(name, dev.stream_handle(device), *args)
 
 
-def _vector(tensor: torch.Tensor, name: str, dtype: torch.dtype, length: int | None = None) -> None:
+def _vector(tensor: torch.Tensor, name: str, dtype: torch.dtype, like: torch.Tensor, length: int | None = None) -> int:
+    """A contiguous vector on ``like``'s device; returns its address."""
+    if (
+        tensor.dtype is dtype
+        and tensor.dim() == 1
+        and tensor.is_contiguous()
+        and tensor.get_device() == like.get_device()
+        and (length is None or tensor.numel() == length)
+    ):
+        return tensor.data_ptr()
+    if tensor.get_device() != like.get_device():
+        raise _misplaced(tensor, name, like)
     dev.require_dtype(tensor, name, dtype)
-    if tensor.ndim != 1 or not tensor.is_contiguous():
+    if tensor.dim() != 1 or not tensor.is_contiguous():
         raise ValueError(f"{name} must be a contiguous vector")
-    if length is not None and tensor.shape[0] != length:
-        raise ValueError(f"{name} must have {length} entries, got {tensor.shape[0]}")
+    raise ValueError(f"{name} must have {length} entries, got {tensor.numel()}")
+
+
+def _block_table(table: torch.Tensor, n: int, like: torch.Tensor) -> tuple[int, int]:
+    """(row stride, blocks a row) of an int32 table with a row for each of n requests."""
+    if table.get_device() != like.get_device():
+        raise _misplaced(table, "block_table", like)
+    if table.dtype is not torch.int32:
+        dev.require_dtype(table, "block_table", torch.int32)
+    if table.dim() != 2:
+        raise ValueError("block_table must be [requests, max_blocks] with contiguous rows")
+    (rows, blocks), (stride, inner) = table.shape, table.stride()
+    if rows < n or (blocks > 1 and inner != 1):
+        raise ValueError("block_table must be [requests, max_blocks] with contiguous rows and a row for every request")
+    return (stride if rows > 1 else blocks), blocks
 
 
 # ------------------------------------------------------------------ tables --
@@ -89,69 +115,65 @@ def build_step_tables(
     -1 and position 0, rows of the tables behind request n stay as they were.
     ``max_query_len`` (the longest request's new tokens, if the host knows it)
     only sizes the launch."""
-    device = computed_tokens.device
-    _same_device(
-        device, computed_tokens=computed_tokens, new_tokens=new_tokens, request_offsets=request_offsets, block_ids=block_ids,
-        block_offsets=block_offsets, query_start_loc=query_start_loc, seq_lens=seq_lens, positions=positions,
-        slot_mapping=slot_mapping, block_table=block_table,
-    )
-    _vector(computed_tokens, "computed_tokens", torch.int32)
-    n = computed_tokens.shape[0]
-    _vector(new_tokens, "new_tokens", torch.int32, n)
-    if request_offsets is not None:
-        _vector(request_offsets, "request_offsets", torch.int64, n)
-    _vector(block_ids, "block_ids", torch.int64)
-    _vector(block_offsets, "block_offsets", torch.int64, n + 1)
-    _vector(query_start_loc, "query_start_loc", torch.int32, n + 1)
-    _vector(seq_lens, "seq_lens", torch.int32)
-    if seq_lens.shape[0] < n:
+    dev.require_hip(computed_tokens, "computed_tokens")
+    like = computed_tokens
+    n = computed_tokens.numel()
+    computed = _vector(computed_tokens, "computed_tokens", torch.int32, like)
+    new = _vector(new_tokens, "new_tokens", torch.int32, like, n)
+    offsets = None if request_offsets is None else _vector(request_offsets, "request_offsets", torch.int64, like, n)
+    ids = _vector(block_ids, "block_ids", torch.int64, like)
+    id_offsets = _vector(block_offsets, "block_offsets", torch.int64, like, n + 1)
+    start = _vector(query_start_loc, "query_start_loc", torch.int32, like, n + 1)
+    lens = _vector(seq_lens, "seq_lens", torch.int32, like)
+    if seq_lens.numel() < n:
         raise ValueError("seq_lens must have an entry for every request")
-    _vector(positions, "positions", torch.int64)
-    tokens = positions.shape[0]
-    _vector(slot_mapping, "slot_mapping", torch.int64, tokens)
-    dev.require_dtype(block_table, "block_table", torch.int32)
-    if block_table.ndim != 2 or block_table.shape[0] < n or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
-        raise ValueError("block_table must be [>= requests, max_blocks] with contiguous rows")
-    if max_query_len is not None and max_query_len < 0:
+    tokens = positions.numel()
+    places = _vector(positions, "positions", torch.int64, like)
+    slots = _vector(slot_mapping, "slot_mapping", torch.int64, like, tokens)
+    stride, blocks = _block_table(block_table, n, like)
+    longest = tokens if max_query_len is None else int(max_query_len)
+    if longest < 0:
         raise ValueError("max_query_len must be non-negative")
     _call(
-        device, "kvc_step_tables", n, computed_tokens.data_ptr(), new_tokens.data_ptr(), dev.ptr(request_offsets),
-        block_ids.data_ptr(), block_offsets.data_ptr(), int(page_tokens), int(tokens if max_query_len is None else max_query_len),
-        tokens, block_table.shape[1], _table_stride(block_table),
-        query_start_loc.data_ptr(), seq_lens.data_ptr(), positions.data_ptr(), slot_mapping.data_ptr(), block_table.data_ptr(),
+        like.device, "kvc_step_tables", n, computed, new, offsets, ids, id_offsets, int(page_tokens), longest, tokens, blocks, stride, start,
+        lens, places, slots, block_table.data_ptr(),
     )
 
 
 # ------------------------------------------------------------------ rotary --
 
 
-def _heads(tensor: torch.Tensor, name: str, tokens: int, dim: int, dtype: torch.dtype) -> int:
-    """[tokens, heads, dim] with unit inner stride; returns the head count."""
-    if tensor.ndim != 3 or tensor.shape[0] != tokens or tensor.shape[2] != dim:
-        raise ValueError(f"{name} must have shape [{tokens}, heads, {dim}], got {tuple(tensor.shape)}")
-    if tensor.dtype != dtype:
-        raise ValueError(f"{name} must have the cache's dtype {dtype}, got {tensor.dtype}")
-    if tensor.stride(2) != 1:
+def _heads(tensor: torch.Tensor, name: str, tokens: int, like: torch.Tensor) -> tuple[int, int, int, int]:
+    """[tokens, heads, D] of the cache ``like`` with unit inner stride: (address,
+    token stride, head stride, heads); a dimension of one entry has no stride."""
+    if tensor.get_device() != like.get_device():
+        raise _misplaced(tensor, name, like)
+    shape, dim = tensor.shape, like.shape[3]
+    if len(shape) != 3 or shape[0] != tokens or shape[2] != dim:
+        raise ValueError(f"{name} must have shape [{tokens}, heads, {dim}], got {tuple(shape)}")
+    if tensor.dtype is not like.dtype:
+        raise ValueError(f"{name} must have the cache's dtype {like.dtype}, got {tensor.dtype}")
+    token, head, inner = tensor.stride()
+    if inner != 1:
         raise ValueError(f"{name} must have contiguous heads")
-    return tensor.shape[1]
+    return tensor.data_ptr(), (token if tokens > 1 else 0), (head if shape[1] > 1 else 0), shape[1]
 
 
-def _steps(tensor: torch.Tensor) -> tuple[int, int]:
-    """Token and head strides; a dimension of one entry has none."""
-    tokens, heads, _ = tensor.shape
-    step = tensor.stride()
-    return (step[0] if tokens > 1 else 0), (step[1] if heads > 1 else 0)
-
-
-def _table_stride(table: torch.Tensor) -> int:
-    return table.stride(0) if table.shape[0] > 1 else table.shape[1]
-
-
-def _cache_pair(k_cache: torch.Tensor, v_cache: torch.Tensor) -> None:
-    dev.validate_cache(k_cache, "k_cache")
-    dev.require_hip(v_cache, "v_cache")
-    if v_cache.shape != k_cache.shape or v_cache.stride() != k_cache.stride() or v_cache.dtype != k_cache.dtype:
+def _cache_pair(k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[int, int, int, int, int]:
+    """(dtype code, pages, page stride, KV heads, head dim) of the two caches."""
+    dev.require_hip(k_cache, "k_cache")
+    code, shape, step = _DTYPE_CODES.get(k_cache.dtype), k_cache.shape, k_cache.stride()
+    if code is None or len(shape) != 4:
+        dev.validate_cache(k_cache, "k_cache")
+    pages, block, heads, dim = shape
+    row = heads * dim
+    if block != dev.BLOCK_SIZE or step[1:] != (row, dim, 1) or step[0] < block * row:
+        dev.validate_cache(k_cache, "k_cache")
+    if v_cache.get_device() != k_cache.get_device():
+        raise _misplaced(v_cache, "v_cache", k_cache)
+    if v_cache.dtype is not k_cache.dtype or v_cache.shape != shape or v_cache.stride() != step:
         raise ValueError("K and V caches must share shape, strides and dtype")
+    return code, pages, step[0], heads, dim
 
 
 def rotate_and_store(
@@ -183,32 +205,33 @@ def rotate_and_store(
     [tokens], each slot at most once; tokens with a slot outside the cache (-1)
     store nothing.  Returns the rotated queries: ``q_out`` (may be ``q``) or a
     new tensor."""
-    device = k_cache.device
-    _cache_pair(k_cache, v_cache)
-    _same_device(device, v_cache=v_cache, q=q, k=k, v=v, positions=positions, omega=omega, slot_mapping=slot_mapping, q_out=q_out)
-    _, _, kv_heads, dim = k_cache.shape
+    code, pages, page_stride, kv_heads, dim = _cache_pair(k_cache, v_cache)
     tokens = slot_mapping.numel()
-    _vector(slot_mapping, "slot_mapping", torch.int64)
-    heads = _heads(q, "q", tokens, dim, k_cache.dtype)
-    for name, t in (("k", k), ("v", v)):
-        if _heads(t, name, tokens, dim, k_cache.dtype) != kv_heads:
-            raise ValueError(f"{name} must have the cache's {kv_heads} heads")
+    slots = _vector(slot_mapping, "slot_mapping", torch.int64, k_cache)
+    *q_place, heads = _heads(q, "q", tokens, k_cache)
+    *k_place, k_heads = _heads(k, "k", tokens, k_cache)
+    *v_place, v_heads = _heads(v, "v", tokens, k_cache)
+    if k_heads != kv_heads or v_heads != kv_heads:
+        raise ValueError(f"{'v' if k_heads == kv_heads else 'k'} must have the cache's {kv_heads} heads")
     if q_out is None:
-        q_out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=device)
-    elif _heads(q_out, "q_out", tokens, dim, k_cache.dtype) != heads:
+        q_out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
+    *out_place, out_heads = _heads(q_out, "q_out", tokens, k_cache)
+    if out_heads != heads:
         raise ValueError("q_out must have q's heads")
-    elif q_out.data_ptr() == q.data_ptr() and q_out.stride() != q.stride():
+    if heads and out_place[0] == q_place[0] and out_place != q_place:
         raise ValueError("q_out may be q itself, but not another view of it")
-    _vector(omega, "omega", torch.float32)
-    freq = omega.shape[0]
+    freq = omega.numel()
+    turns = _vector(omega, "omega", torch.float32, k_cache)
     if not 0 < 2 * freq <= dim:
         raise ValueError(f"omega must hold one to head_dim/2 = {dim // 2} frequencies, got {freq}")
-    dev.require_dtype(positions, "positions", torch.int64)
-    if positions.ndim == 1:
-        positions = positions[None]
-    if positions.ndim != 2 or positions.shape[1] != tokens or (tokens > 1 and positions.stride(1) != 1):
+    if positions.get_device() != k_cache.get_device():
+        raise _misplaced(positions, "positions", k_cache)
+    if positions.dtype is not torch.int64:
+        dev.require_dtype(positions, "positions", torch.int64)
+    shape, step = positions.shape, positions.stride()
+    if not 1 <= len(shape) <= 2 or shape[-1] != tokens or (tokens > 1 and step[-1] != 1):
         raise ValueError("positions must be [tokens] or [axes, tokens] with contiguous rows")
-    axes = positions.shape[0]
+    axes, axis_step = (1, 0) if len(shape) == 1 else (shape[0], step[0])
     share = (freq,) if sections is None else tuple(int(x) for x in sections)
     if not 1 <= axes <= 4 or len(share) != axes:
         raise ValueError(f"sections must name the frequencies of each of the {axes} axes (one to four)")
@@ -217,10 +240,9 @@ def rotate_and_store(
     if axis_order not in AXIS_ORDERS:
         raise ValueError(f"axis_order must be one of {', '.join(AXIS_ORDERS)}, got {axis_order!r}")
     _call(
-        device, "kvc_rotate_and_store", dev.cache_dtype_code(k_cache.dtype), dev.rope_style_code(rope_style), tokens, heads, kv_heads,
-        dim, 2 * freq, q.data_ptr(), *_steps(q), k.data_ptr(), *_steps(k), v.data_ptr(), *_steps(v), positions.data_ptr(), positions.stride(0), axes, (ctypes.c_int * axes)(*share), int(axis_order == "cycled"),
-        omega.data_ptr(), slot_mapping.data_ptr(), q_out.data_ptr(), *_steps(q_out), k_cache.data_ptr(),
-        v_cache.data_ptr(), k_cache.shape[0], k_cache.stride(0),
+        k_cache.device, "kvc_rotate_and_store", code, dev.rope_style_code(rope_style), tokens, heads, kv_heads,
+        dim, 2 * freq, *q_place, *k_place, *v_place, positions.data_ptr(), axis_step, axes, (ctypes.c_int * axes)(*share),
+        int(axis_order == "cycled"), turns, slots, *out_place, k_cache.data_ptr(), v_cache.data_ptr(), pages, page_stride,
     )
     return q_out
 
@@ -273,53 +295,44 @@ def attend_paged(
     may not overlap q; rows outside every request are not written.
     ``workspace``: uint8, at least :func:`attend_workspace_bytes`, for callers
     that keep one per stream; calls that overlap in time need one each."""
-    device = k_cache.device
-    _cache_pair(k_cache, v_cache)
-    _same_device(
-        device, v_cache=v_cache, q=q, query_start_loc=query_start_loc, seq_lens=seq_lens, block_table=block_table, out=out,
-        workspace=workspace,
-    )
-    num_pages, _, kv_heads, dim = k_cache.shape
+    code, pages, page_stride, kv_heads, dim = _cache_pair(k_cache, v_cache)
     tokens = q.shape[0]
-    heads = _heads(q, "q", tokens, dim, k_cache.dtype)
+    *q_place, heads = _heads(q, "q", tokens, k_cache)
     if heads == 0 or heads % kv_heads:
         raise ValueError(f"query heads ({heads}) must be a positive multiple of the cache's KV heads ({kv_heads})")
-    _vector(query_start_loc, "query_start_loc", torch.int32)
-    n = query_start_loc.shape[0] - 1
+    n = query_start_loc.numel() - 1
+    start = _vector(query_start_loc, "query_start_loc", torch.int32, k_cache)
     if n < 0:
         raise ValueError("query_start_loc must have one entry more than there are requests")
-    _vector(seq_lens, "seq_lens", torch.int32)
-    dev.require_dtype(block_table, "block_table", torch.int32)
-    if block_table.ndim != 2 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
-        raise ValueError("block_table must be [requests, max_blocks] with contiguous rows")
-    if seq_lens.shape[0] < n or block_table.shape[0] < n:
-        raise ValueError("seq_lens and block_table must have a row for every request")
-    max_blocks = block_table.shape[1]
-    longest = tokens if max_query_len is None else int(max_query_len)
-    reach = max_blocks * dev.BLOCK_SIZE if max_seq_len is None else min(int(max_seq_len), max_blocks * dev.BLOCK_SIZE)
+    lens = _vector(seq_lens, "seq_lens", torch.int32, k_cache)
+    if seq_lens.numel() < n:
+        raise ValueError("seq_lens must have a row for every request")
+    stride, blocks = _block_table(block_table, n, k_cache)
+    longest = tokens if max_query_len is None else min(int(max_query_len), tokens)
+    reach = blocks * dev.BLOCK_SIZE if max_seq_len is None else min(int(max_seq_len), blocks * dev.BLOCK_SIZE)
     if longest < 0 or reach < 0:
         raise ValueError("max_query_len and max_seq_len must be non-negative")
-    longest = min(longest, tokens)
     factor = dim**-0.5 if scale is None else float(scale)
     if not (factor > 0 and math.isfinite(factor)):
         raise ValueError("scale must be positive and finite")
     if window < 0 or sinks < 0:
         raise ValueError("window and sinks must be non-negative")
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=device)
-    elif _heads(out, "out", tokens, dim, k_cache.dtype) != heads:
+        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
+    *out_place, out_heads = _heads(out, "out", tokens, k_cache)
+    if out_heads != heads:
         raise ValueError("out must have q's shape")
-    bytes_needed = attend_workspace_bytes(heads, kv_heads, dim, n, tokens, longest, reach)
+    size = attend_workspace_bytes(heads, kv_heads, dim, n, tokens, longest, reach)
     if workspace is None:
-        workspace = torch.empty(bytes_needed, dtype=torch.uint8, device=device)
-    elif not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < bytes_needed:
-        raise ValueError(f"workspace must be contiguous and hold at least {bytes_needed} bytes")
+        workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+    elif workspace.get_device() != k_cache.get_device():
+        raise _misplaced(workspace, "workspace", k_cache)
+    elif not workspace.is_contiguous() or workspace.nbytes < size:
+        raise ValueError(f"workspace must be contiguous and hold at least {size} bytes")
     most = (1 << 31) - 1
     _call(
-        device, "kvc_attend_paged", dev.cache_dtype_code(k_cache.dtype), q.data_ptr(), *_steps(q), k_cache.data_ptr(),
-        v_cache.data_ptr(), num_pages, k_cache.stride(0), kv_heads, heads // kv_heads, dim, n, tokens, query_start_loc.data_ptr(),
-        seq_lens.data_ptr(), block_table.data_ptr(), _table_stride(block_table),
-        max_blocks, longest, reach, factor, min(int(window), most), min(int(sinks), most), out.data_ptr(), *_steps(out),
-        workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+        k_cache.device, "kvc_attend_paged", code, *q_place, k_cache.data_ptr(), v_cache.data_ptr(), pages,
+        page_stride, kv_heads, heads // kv_heads, dim, n, tokens, start, lens, block_table.data_ptr(), stride, blocks, longest, reach,
+        factor, min(int(window), most), min(int(sinks), most), *out_place, workspace.data_ptr(), workspace.nbytes,
     )
     return out
