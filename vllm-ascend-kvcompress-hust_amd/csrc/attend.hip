@@ -29,8 +29,7 @@ AttendPlan make_plan(int kv_heads, int qpk, int head_dim, int n_seq, int64_t num
     p.row_tiles = most_rows <= kFewRows ? 1 : kFewTilesMost;
     p.sequences = n_seq < kFewSequences ? n_seq : kFewSequences;
     const int64_t bound = static_cast<int64_t>(p.sequences) * kv_heads * pages;
-    // Workgroups that fit the device at once: 3 or 2 a compute unit by their LDS.
-    const int64_t resident = kCompute * (dim <= 128 ? 3 : 2);
+    const int64_t resident = kCompute * few_residents(dim, p.row_tiles);
     p.workgroups = static_cast<int>(bound < resident ? bound : resident);
     few = static_cast<size_t>(p.workgroups) * (16 + 8 * piece_floats(kFewRows * p.row_tiles, dim));
   }

@@ -14,6 +14,8 @@
 // order; V passes through the wave's own LDS, where ds_read_b64_tr_b16 turns
 // rows into columns.
 
+#include <type_traits>
+
 #include "attend_internal.h"
 
 namespace kvc {
@@ -40,12 +42,11 @@ struct FewLayout {
   __device__ __forceinline__ static int chunk_at(int to, int i) { return (to ^ (turn(i * kStep) << 5)) + i * kStep * kRow * 2; }
 };
 
-// Waves a SIMD: as many as the registers of a variant's outputs, queries and
-// one slice's K and V leave room for.
-constexpr int few_waves(int dp, int nq) { return dp <= 64 ? (nq == 1 ? 4 : 3) : (dp <= 128 ? (nq == 1 ? 3 : 2) : (nq == 1 ? 2 : 1)); }
-
+// Workgroups of a compute unit (waves of a SIMD): as many as leave registers for
+// the outputs, the queries, and a slice's K and V ahead of their use; each wave
+// then has 64 x DP bytes in flight.
 template <bool F16, int DP, int NQ>
-__global__ __launch_bounds__(kFewThreads, few_waves(DP, NQ)) void attend_few_kernel(AttendArgs a) {
+__global__ __launch_bounds__(kFewThreads, few_residents(DP, NQ)) void attend_few_kernel(AttendArgs a) {
   typedef AttendElem<F16> E;
   typedef typename E::vec vec_t;
   constexpr int kSteps = DP / 32;   // 32-dim steps of K Q^T
@@ -118,7 +119,7 @@ __global__ __launch_bounds__(kFewThreads, few_waves(DP, NQ)) void attend_few_ker
   while (at < range_end) {
     while (before[r + 1] <= at) ++r;
     r = uniform(r);
-    const Request s = request_of(a, r);
+    const Request s = uniform_request_of(a, r);
     const TileRange pages = tile_range<kBlockShift>(a, s, s.len - s.fresh, s.len - 1);
     const int request_begin = uniform(before[r]);
     const int tiles = (uniform(before[r + 1]) - request_begin) / a.kv_heads;
@@ -170,7 +171,7 @@ __global__ __launch_bounds__(kFewThreads, few_waves(DP, NQ)) void attend_few_ker
         const int block = pages.tile(f.tile);
         f.key0 = (block << kBlockShift) + wave * kSliceKeys;
         if (f.key0 >= last_end || (f.key0 + kSliceKeys <= first_low && f.key0 >= a.sinks)) continue;
-        const int page = uniform(table[block]);
+        const int page = scalar_at(table, block);
         if (page < 0 || page >= a.num_pages) continue;
         f.base = page * a.page_stride + static_cast<int64_t>(wave * kSliceKeys) * row_elems + head * a.head_dim;
         break;
@@ -200,8 +201,10 @@ __global__ __launch_bounds__(kFewThreads, few_waves(DP, NQ)) void attend_few_ker
     float m_run[NQ], l_run[NQ];
     // Weights of zero, and second words of any sign, turn an infinity or NaN
     // among V into NaN for rows that do not see it.  That shows in the outputs:
-    // a wave that finds one there goes over its keys again with care.
-    for (bool careful = false;; careful = true) {
+    // a wave that finds one there goes over its keys again with care.  Returns
+    // whether there is one.
+    auto go_over = [&](auto care) {
+    constexpr bool careful = decltype(care)::value;
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
       m_run[n] = kNegInf;
@@ -283,7 +286,7 @@ __global__ __launch_bounds__(kFewThreads, few_waves(DP, NQ)) void attend_few_ker
         const s16x4 v0 = read_column(from);
         const s16x4 v1 = read_column(from + 16 * Layout::kRow * 2);
         vec_t vf = join_columns<vec_t>(v0, v1);
-        if (careful) {
+        if constexpr (careful) {
           // Values that are not finite are added only to the rows that see them,
           // token by token, by the first word of their weights.
           s16x8 raw = __builtin_bit_cast(s16x8, vf), odd = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -327,8 +330,9 @@ __global__ __launch_bounds__(kFewThreads, few_waves(DP, NQ)) void attend_few_ker
       for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
         for (int i = 0; i < 4; ++i) wild |= !(fabsf(acc[n][b][i]) <= 3.4e38f);
-    if (careful || !__any(wild)) break;
-    }
+    return wild;
+    };
+    if (__any(go_over(std::false_type{}))) go_over(std::true_type{});
 
     // Join the four waves: a common maximum, then sums.
 #pragma unroll
@@ -418,48 +422,36 @@ __global__ __launch_bounds__(kFewThreads, few_waves(DP, NQ)) void attend_few_ker
 }
 
 // Joins the pieces of the (request, head) that begins in workgroup blockIdx.x
-// and ends in a later one: out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.
+// and ends in a later one, four rows a workgroup:
+// out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.
 template <bool F16, int DP, int NQ>
 __global__ __launch_bounds__(kFewThreads) void attend_few_join_kernel(AttendArgs a) {
   typedef AttendElem<F16> E;
   constexpr int kRows = 16 * NQ;
-  const int wg = blockIdx.x;
-  const int count = a.header[4 * wg + 2];
+  const int wg = blockIdx.x, row0 = blockIdx.y * 4;
+  const int count = scalar_at(a.header, 4 * wg + 2);
   if (count < 2) return;
-  const int r = a.header[4 * wg], head = a.header[4 * wg + 1], kind = a.header[4 * wg + 3];
-  const Request s = request_of(a, r);
+  const int r = scalar_at(a.header, 4 * wg), head = scalar_at(a.header, 4 * wg + 1), kind = scalar_at(a.header, 4 * wg + 3);
+  const Request s = uniform_request_of(a, r);
   const int rows = s.fresh * a.qpk;
+  if (row0 >= rows) return;
   const int64_t size = piece_floats(kRows, DP);
   const float* const first = a.partial + (2 * static_cast<int64_t>(wg) + kind) * size;
   const float* const rest = a.partial + 2 * static_cast<int64_t>(wg) * size;  // piece i > 0 at 2*i*size
-  for (int u = threadIdx.x; u < rows * (DP / 4); u += kFewThreads) {
-    const int m = u / (DP / 4), d = (u - m * (DP / 4)) * 4;
-    if (d >= a.head_dim) continue;
-    float top = kNegInf;
-    for (int i = 0; i < count; ++i) top = fmaxf(top, (i ? rest + 2 * i * size : first)[kRows * DP + 2 * m]);
-    const float use = top == kNegInf ? 0.0f : top;
-    f32x4 sum = {0, 0, 0, 0};
-    float l = 0.0f;
-#pragma unroll 4
-    for (int i = 0; i < count; ++i) {
-      const float* p = i ? rest + 2 * i * size : first;
-      const f32x2 ml = *reinterpret_cast<const f32x2*>(p + kRows * DP + 2 * m);
-      const float w = exp2_fast(ml.x - use);
-      sum += *reinterpret_cast<const f32x4*>(p + m * DP + d) * w;
-      l += ml.y * w;
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const int token = m / a.qpk, g = m - token * a.qpk;
-    uint16_t* to = a.out + (s.token0 + token) * a.out_token_stride + (head * a.qpk + g) * a.out_head_stride;
-    *gptr(reinterpret_cast<u32x2*>(to + d)) = u32x2{E::pack(sum[0] * inv, sum[1] * inv), E::pack(sum[2] * inv, sum[3] * inv)};
-  }
+  join_pieces<DP>(
+      count, row0, rows, a.head_dim, kRows * DP, [&](int i) { return i ? rest + 2 * i * size : first; },
+      [&](int m, int d, f32x4 x) {
+        const int token = m / a.qpk, g = m - token * a.qpk;
+        uint16_t* to = a.out + (s.token0 + token) * a.out_token_stride + (head * a.qpk + g) * a.out_head_stride;
+        *gptr(reinterpret_cast<u32x2*>(to + d)) = u32x2{E::pack(x[0], x[1]), E::pack(x[2], x[3])};
+      });
 }
 
 template <bool F16, int DP, int NQ>
 int launch(hipStream_t stream, const AttendArgs& a, int workgroups) {
   attend_few_kernel<F16, DP, NQ><<<workgroups, kFewThreads, 0, stream>>>(a);
   if (int rc = launch_status("kvc_attend_paged")) return rc;
-  if (workgroups > 1) attend_few_join_kernel<F16, DP, NQ><<<workgroups, kFewThreads, 0, stream>>>(a);
+  if (workgroups > 1) attend_few_join_kernel<F16, DP, NQ><<<dim3(workgroups, 4 * NQ), kFewThreads, 0, stream>>>(a);
   return launch_status("kvc_attend_paged");
 }
 

@@ -38,25 +38,38 @@ struct AttendArgs {
   int few_rows;  // requests of at most this many rows are the few-rows kernel's
 };
 
+// An entry of a table that the launch only reads, by a scalar load: a vector one
+// would wait for every key and value in flight.
+__device__ __forceinline__ int scalar_at(const int32_t* p, int64_t i) {
+  return ((__attribute__((address_space(4))) const int32_t*)p)[i];
+}
+
 // One request's rows and keys.
 struct Request {
   int token0, fresh;  // first token, new tokens
   int len, keys;      // cached tokens; those that the block table covers
 };
 
-__device__ __forceinline__ Request request_of(const AttendArgs& a, int r) {
+__device__ __forceinline__ Request request_from(const AttendArgs& a, int start0, int start1, int len) {
   Request s;
   const int64_t total = a.num_tokens;
-  int64_t t0 = a.start[r], t1 = a.start[r + 1];
+  int64_t t0 = start0, t1 = start1;
   t0 = t0 < 0 ? 0 : (t0 > total ? total : t0);
   t1 = t1 < t0 ? t0 : (t1 > total ? total : t1);
   s.token0 = static_cast<int>(t0);
   s.fresh = static_cast<int>(t1 - t0);
-  const int len = a.seq_lens[r];
   s.len = len < 0 ? 0 : len;
   const int64_t most = static_cast<int64_t>(a.max_blocks) << kBlockShift;
   s.keys = s.len < most ? s.len : static_cast<int>(most);
   return s;
+}
+
+// Of a request that differs from lane to lane, and of one that does not.
+__device__ __forceinline__ Request request_of(const AttendArgs& a, int r) {
+  return request_from(a, a.start[r], a.start[r + 1], a.seq_lens[r]);
+}
+__device__ __forceinline__ Request uniform_request_of(const AttendArgs& a, int r) {
+  return request_from(a, scalar_at(a.start, r), scalar_at(a.start, r + 1), scalar_at(a.seq_lens, r));
 }
 
 // Key tiles of 2^SHIFT keys that rows at places [first, last] see: the first
@@ -133,6 +146,58 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 
 constexpr float kNegInf = -__builtin_inff();
 
+// Joins `count` pieces of four rows (first, first + 1, .. below `rows`) of which
+// piece i is at piece(i): `floats` unnormalised outputs of DP dims a row, then
+// (maximum, sum) pairs.  A workgroup of 256: a wave a row finds the common
+// maximum and sum, then every thread adds four dims of some of the pieces, and
+// the shares meet in LDS.  store(row, dim, f32x4) takes the results.
+template <int DP, typename Piece, typename Store>
+__device__ __forceinline__ void join_pieces(int count, int first, int rows, int head_dim, int floats, Piece piece, Store store) {
+  constexpr int kUnits = DP;  // four rows of DP / 4 units
+  constexpr int kShares = kUnits <= 128 ? 2 : 1;
+  __shared__ float top_of[4], inv_of[4];
+  __shared__ f32x4 shared_sum[kShares > 1 ? 256 : 1];
+  const int lane = threadIdx.x & 63, own = first + (threadIdx.x >> 6);
+  if (own < rows) {
+    float top = kNegInf;
+    for (int i = lane; i < count; i += 64) top = fmaxf(top, piece(i)[floats + 2 * own]);
+#pragma unroll
+    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    const float use = top == kNegInf ? 0.0f : top;
+    float sum = 0.0f;
+    for (int i = lane; i < count; i += 64) {
+      const f32x2 ml = *reinterpret_cast<const f32x2*>(piece(i) + floats + 2 * own);
+      sum += ml[1] * exp2_fast(ml[0] - use);
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+    if (lane == 0) {
+      top_of[own - first] = use;
+      inv_of[own - first] = sum == 0.0f ? 0.0f : 1.0f / sum;
+    }
+  }
+  __syncthreads();
+  const int share = threadIdx.x / kUnits, unit = threadIdx.x - share * kUnits;
+  const int local = unit / (DP / 4), d = (unit - local * (DP / 4)) * 4, row = first + local;
+  const bool working = share < kShares && row < rows && d < head_dim;
+  f32x4 sum = {0, 0, 0, 0};
+  if (working) {
+    const float use = top_of[local];
+#pragma unroll 8
+    for (int i = share; i < count; i += kShares) {
+      const float* p = piece(i);
+      sum += *reinterpret_cast<const f32x4*>(p + row * DP + d) * exp2_fast(p[floats + 2 * row] - use);
+    }
+    sum *= inv_of[local];
+  }
+  if constexpr (kShares > 1) {
+    if (share == 1) shared_sum[unit] = sum;
+    __syncthreads();
+    if (share == 0) sum += shared_sum[unit];
+  }
+  if (working && share == 0) store(row, d, sum);
+}
+
 // Entry points of the kernels' files.
 int launch_attend_few(hipStream_t stream, bool f16, const AttendArgs& a, int workgroups, int row_tiles);
 int launch_attend_many(hipStream_t stream, bool f16, const AttendArgs& a, int64_t tiles, int splits);
@@ -142,6 +207,9 @@ constexpr int kFewRows = 16;         // rows of one few-rows tile
 constexpr int kFewTilesMost = 2;     // tiles of a request that the few-rows kernel takes
 constexpr int kFewSequences = 1024;  // requests of one launch (their prefix sums sit in LDS)
 constexpr int kManyRows = 128;       // rows of one many-rows tile
+
+// Few-rows workgroups that a compute unit holds.
+constexpr int few_residents(int dim, int row_tiles) { return dim <= 64 ? 4 - row_tiles : (dim <= 128 ? 2 : 1); }
 
 // Floats of a piece of `rows` rows: unnormalised outputs, then (max, sum) pairs.
 __host__ __device__ inline int64_t piece_floats(int rows, int dim) { return static_cast<int64_t>(rows) * (dim + 2); }

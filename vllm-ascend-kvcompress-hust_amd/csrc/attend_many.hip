@@ -13,6 +13,8 @@
 // error of a sum of them is that of one rounding, as the output's own is); the
 // maxima, sums and outputs stay in float32.
 
+#include <type_traits>
+
 #include "attend_internal.h"
 
 namespace kvc {
@@ -46,7 +48,7 @@ struct ManyTile {
 };
 
 __device__ __forceinline__ int64_t tile_base(const AttendArgs& a, int r) {
-  int64_t t = a.start[r];
+  int64_t t = scalar_at(a.start, r);
   t = t < 0 ? 0 : (t > a.num_tokens ? a.num_tokens : t);
   return t * a.qpk / kManyRows + r;
 }
@@ -80,7 +82,7 @@ __global__ __launch_bounds__(kManyThreads, DP <= 128 ? 2 : 1) void attend_many_k
   const int split = rest % splits;
   const int64_t tile = tiles - 1 - rest / splits;  // the last rows see the most keys: they begin first
   const ManyTile mine = tile_of(a, tile);
-  const Request s = request_of(a, mine.request);
+  const Request s = uniform_request_of(a, mine.request);
   const int64_t all_rows = static_cast<int64_t>(s.fresh) * a.qpk;
   if (mine.row0 >= all_rows || all_rows <= a.few_rows) return;
   const int rows = static_cast<int>(all_rows);
@@ -132,7 +134,7 @@ __global__ __launch_bounds__(kManyThreads, DP <= 128 ? 2 : 1) void attend_many_k
   bool next_valid = false;
   auto load = [&](int t) {
     const int key0 = range.tile(t) << L::kShift;
-    const int page = uniform(table[key0 >> kBlockShift]);
+    const int page = scalar_at(table, key0 >> kBlockShift);
     next_valid = page >= 0 && page < a.num_pages;
     if (!next_valid) return;
     const int64_t base = page * a.page_stride + static_cast<int64_t>(key0 & (kBlockSize - 1)) * row_elems + head * a.head_dim;
@@ -150,8 +152,9 @@ __global__ __launch_bounds__(kManyThreads, DP <= 128 ? 2 : 1) void attend_many_k
   float m_run, l_run;
   // A weight of zero turns an infinity or NaN among V into NaN for rows that do
   // not see it.  That shows in the outputs: a workgroup that finds one there
-  // goes over its keys again with care.
-  for (bool careful = false;; careful = true) {
+  // goes over its keys again with care.  Returns whether the thread has one.
+  auto go_over = [&](auto care) {
+  constexpr bool careful = decltype(care)::value;
 #pragma unroll
   for (int b = 0; b < kBlocks; ++b) acc[b] = f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
   m_run = kNegInf;
@@ -235,7 +238,7 @@ __global__ __launch_bounds__(kManyThreads, DP <= 128 ? 2 : 1) void attend_many_k
           const s16x4 v0 = read_column(at);
           const s16x4 v1 = read_column(at + 8 * L::kBytes);
           vec_t vf = join_columns<vec_t>(v0, v1);
-          if (careful) {
+          if constexpr (careful) {
             // Values that are not finite are added only to the rows that see
             // them, token by token.
             s16x8 raw = __builtin_bit_cast(s16x8, vf), odd = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -269,8 +272,9 @@ __global__ __launch_bounds__(kManyThreads, DP <= 128 ? 2 : 1) void attend_many_k
   for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
     for (int i = 0; i < 16; ++i) wild |= !(fabsf(acc[b][i]) <= 3.4e38f);
-  if (careful || !__syncthreads_or(wild)) break;
-  }
+  return wild;
+  };
+  if (__syncthreads_or(go_over(std::false_type{}))) go_over(std::true_type{});
 
   const float l_all = l_run + __shfl_xor(l_run, 32);
   if (!inside) return;
@@ -299,38 +303,26 @@ __global__ __launch_bounds__(kManyThreads, DP <= 128 ? 2 : 1) void attend_many_k
   }
 }
 
-// Joins the splits of a (row tile, KV head).
+// Joins the splits of a (row tile, KV head), four rows a workgroup.
 template <bool F16, int DP>
 __global__ __launch_bounds__(kManyThreads) void attend_many_join_kernel(AttendArgs a, int splits) {
   typedef AttendElem<F16> E;
-  const int head = blockIdx.x % a.kv_heads;
+  const int head = blockIdx.x % a.kv_heads, row0 = blockIdx.y * 4;
   const int64_t tile = blockIdx.x / a.kv_heads;
   const ManyTile mine = tile_of(a, tile);
-  const Request s = request_of(a, mine.request);
+  const Request s = uniform_request_of(a, mine.request);
   const int64_t all_rows = static_cast<int64_t>(s.fresh) * a.qpk;
-  if (mine.row0 >= all_rows || all_rows <= a.few_rows) return;
+  if (mine.row0 + row0 >= all_rows || all_rows <= a.few_rows) return;
   const int rows = all_rows - mine.row0 < kManyRows ? static_cast<int>(all_rows - mine.row0) : kManyRows;
   const int64_t size = piece_floats(kManyRows, DP);
   const float* const pieces = a.partial + (tile * a.kv_heads + head) * splits * size;
-  for (int u = threadIdx.x; u < rows * (DP / 4); u += kManyThreads) {
-    const int local = u / (DP / 4), d = (u - local * (DP / 4)) * 4;
-    if (d >= a.head_dim) continue;
-    float top = kNegInf;
-    for (int i = 0; i < splits; ++i) top = fmaxf(top, pieces[i * size + kManyRows * DP + 2 * local]);
-    const float use = top == kNegInf ? 0.0f : top;
-    f32x4 sum = {0, 0, 0, 0};
-    float l = 0.0f;
-    for (int i = 0; i < splits; ++i) {
-      const f32x2 ml = *reinterpret_cast<const f32x2*>(pieces + i * size + kManyRows * DP + 2 * local);
-      const float w = exp2_fast(ml.x - use);
-      sum += *reinterpret_cast<const f32x4*>(pieces + i * size + local * DP + d) * w;
-      l += ml.y * w;
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const int m = mine.row0 + local, token = m / a.qpk, g = m - token * a.qpk;
-    uint16_t* to = a.out + (s.token0 + token) * a.out_token_stride + (head * a.qpk + g) * a.out_head_stride;
-    *gptr(reinterpret_cast<u32x2*>(to + d)) = u32x2{E::pack(sum[0] * inv, sum[1] * inv), E::pack(sum[2] * inv, sum[3] * inv)};
-  }
+  join_pieces<DP>(
+      splits, row0, rows, a.head_dim, kManyRows * DP, [&](int i) { return pieces + i * size; },
+      [&](int local, int d, f32x4 x) {
+        const int m = mine.row0 + local, token = m / a.qpk, g = m - token * a.qpk;
+        uint16_t* to = a.out + (s.token0 + token) * a.out_token_stride + (head * a.qpk + g) * a.out_head_stride;
+        *gptr(reinterpret_cast<u32x2*>(to + d)) = u32x2{E::pack(x[0], x[1]), E::pack(x[2], x[3])};
+      });
 }
 
 template <bool F16, int DP>
@@ -339,7 +331,8 @@ int launch(hipStream_t stream, const AttendArgs& a, int64_t tiles, int splits) {
       <<<static_cast<unsigned>(tiles * a.kv_heads * splits), kManyThreads, 0, stream>>>(a, tiles, splits);
   if (int rc = launch_status("kvc_attend_paged")) return rc;
   if (splits > 1)
-    attend_many_join_kernel<F16, DP><<<static_cast<unsigned>(tiles * a.kv_heads), kManyThreads, 0, stream>>>(a, splits);
+    attend_many_join_kernel<F16, DP>
+        <<<dim3(static_cast<unsigned>(tiles * a.kv_heads), kManyRows / 4), kManyThreads, 0, stream>>>(a, splits);
   return launch_status("kvc_attend_paged");
 }
 
