@@ -151,6 +151,7 @@ __global__ __launch_bounds__(kFewThreads, few_residents(DP, NQ)) void attend_few
         qf[n][st] = __builtin_bit_cast(vec_t, w);
       }
     }
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // the queries are there: the loop's waits count its own loads alone
     // Keys that some row sees, and those that every row sees.
     const int last_end = place0 + s.fresh < s.keys ? place0 + s.fresh : s.keys;
     const int first_end = place0 + 1 < s.keys ? place0 + 1 : s.keys;
@@ -164,6 +165,7 @@ __global__ __launch_bounds__(kFewThreads, few_residents(DP, NQ)) void attend_few
       int64_t base;
     };
     const int32_t* const table = a.table + r * a.table_stride;
+    PageIds ids;
     auto find = [&](int t) {
       Slice f = {t, 0, 0};
       if (pages.count() == 0) f.tile = piece_last;
@@ -171,7 +173,7 @@ __global__ __launch_bounds__(kFewThreads, few_residents(DP, NQ)) void attend_few
         const int block = pages.tile(f.tile);
         f.key0 = (block << kBlockShift) + wave * kSliceKeys;
         if (f.key0 >= last_end || (f.key0 + kSliceKeys <= first_low && f.key0 >= a.sinks)) continue;
-        const int page = scalar_at(table, block);
+        const int page = ids.at(table, a.max_blocks, block);
         if (page < 0 || page >= a.num_pages) continue;
         f.base = page * a.page_stride + static_cast<int64_t>(wave * kSliceKeys) * row_elems + head * a.head_dim;
         break;
@@ -246,13 +248,16 @@ __global__ __launch_bounds__(kFewThreads, few_residents(DP, NQ)) void attend_few
       for (int n = 0; n < NQ; ++n) {
         float x[8], top = kNegInf;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          x[j] = sc[n][j >> 2][j & 3] * a.scale_log2;
-          if (!whole && !sees(sight[n], a.sinks, key0 + 16 * (j >> 2) + 4 * group + (j & 3))) x[j] = kNegInf;
-          top = fmaxf(top, x[j]);
+        for (int j = 0; j < 8; ++j) x[j] = sc[n][j >> 2][j & 3] * a.scale_log2;
+        if (!whole) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            x[j] = sees(sight[n], a.sinks, key0 + 16 * (j >> 2) + 4 * group + (j & 3)) ? x[j] : kNegInf;
         }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, x[j]);
         top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
+        top = max_across_halves(top);
         const float m_new = fmaxf(m_run[n], top);
         const float m_use = m_new == kNegInf ? 0.0f : m_new;
         const float scale = exp2_fast(m_run[n] - m_use);

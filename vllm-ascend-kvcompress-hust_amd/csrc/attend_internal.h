@@ -105,7 +105,7 @@ __device__ __forceinline__ RowSight sight_of(const AttendArgs& a, const Request&
 }
 
 __device__ __forceinline__ bool sees(const RowSight& s, int sinks, int key) {
-  return key < s.end && (key >= s.low || key < sinks);
+  return (key < s.end) & ((key >= s.low) | (key < sinks));  // no branches: 8 to 32 keys a lane ask
 }
 
 // The element type of a cache for the 32x32 products.
@@ -136,6 +136,27 @@ __device__ __forceinline__ V join_columns(s16x4 a, s16x4 b) {
 
 // A value that every lane holds alike, as a scalar.
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// A request's pages, 64 at a time in the wave's lanes: a page's number then costs
+// no wait.  -1 where the table ends.
+struct PageIds {
+  int first = -(1 << 30), ids = -1;
+  __device__ __forceinline__ int at(const int32_t* table, int max_blocks, int block) {
+    if (block - first >= 64 || block < first) {
+      first = block;
+      const int mine = block + static_cast<int>(threadIdx.x & 63);
+      ids = mine < max_blocks ? *gptr(table + mine) : -1;
+      asm volatile("" : "+v"(ids));  // waited for here, not wherever it is used
+    }
+    return __builtin_amdgcn_readlane(ids, block - first);
+  }
+};
+
+// The larger of a lane's value and that of the lane 32 away.
+__device__ __forceinline__ float max_across_halves(float x) {
+  const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+}
 
 // A buffer of `bytes` bytes for loads with lane offsets; past its end they give zeros.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t page_rsrc(const uint16_t* base, uint32_t bytes) {

@@ -103,8 +103,7 @@ __global__ __launch_bounds__(kManyThreads, DP <= 128 ? 2 : 1) void attend_many_k
   if (!inside) sight.end = 0;
   // The wave's first and last rows' sights.
   const int m_first = mine.row0 + wave * 32, m_last = m_first + 31 < rows ? m_first + 31 : rows - 1;
-  const bool wave_rows = m_first < rows;
-  const int token_first = m_first / a.qpk, token_last = (wave_rows ? m_last : m_first) / a.qpk;
+  const int token_first = m_first / a.qpk, token_last = (m_first < rows ? m_last : m_first) / a.qpk;
   const RowSight first = sight_of(a, s, place0 + token_first), last = sight_of(a, s, place0 + token_last);
 
   vec_t qf[kSteps];
@@ -131,16 +130,20 @@ __global__ __launch_bounds__(kManyThreads, DP <= 128 ? 2 : 1) void attend_many_k
   const int v_row = 4 * half + ((lane & 15) >> 2);
   const int v_from = v_row * L::kBytes + L::v_turn(v_row) + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
   u32x4 kst[L::kLoads], vst[L::kLoads];
-  bool next_valid = false;
+  // The queries are there before the first tile is asked for: the loop's waits
+  // then count its own loads alone.
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  PageIds pages;
+  bool next_there = false;
+  // Zeros from behind the last tile, from pages outside the pool and from behind
+  // the request's last row, whatever the page holds there.
   auto load = [&](int t) {
-    const int key0 = range.tile(t) << L::kShift;
-    const int page = scalar_at(table, key0 >> kBlockShift);
-    next_valid = page >= 0 && page < a.num_pages;
-    if (!next_valid) return;
-    const int64_t base = page * a.page_stride + static_cast<int64_t>(key0 & (kBlockSize - 1)) * row_elems + head * a.head_dim;
-    // Zeros from behind the request's last row, whatever the page holds there.
+    const int key0 = range.tile(t < t_end ? t : t_end - 1) << L::kShift;
+    const int page = pages.at(table, a.max_blocks, key0 >> kBlockShift);
+    next_there = (t < t_end) & (page >= 0) & (page < a.num_pages);
+    const int64_t base = (next_there ? page : 0) * a.page_stride + static_cast<int64_t>(key0 & (kBlockSize - 1)) * row_elems + head * a.head_dim;
     const int left = s.keys - key0 < L::kKeys ? s.keys - key0 : L::kKeys;
-    const uint32_t bytes = (left - 1) * row_bytes + a.head_dim * 2;
+    const uint32_t bytes = next_there ? (left - 1) * row_bytes + a.head_dim * 2 : 0;
     const auto k_page = page_rsrc(a.k + base, bytes), v_page = page_rsrc(a.v + base, bytes);
 #pragma unroll
     for (int i = 0; i < L::kLoads; ++i) kst[i] = __builtin_amdgcn_raw_buffer_load_b128(k_page, from, i * L::kStep * row_bytes, 0);
@@ -163,20 +166,16 @@ __global__ __launch_bounds__(kManyThreads, DP <= 128 ? 2 : 1) void attend_many_k
   for (int t = t_begin; t < t_end; ++t) {
     char* const kt = reinterpret_cast<char*>(k_tile[t & 1]);
     char* const vt = reinterpret_cast<char*>(v_tile[t & 1]);
-    const bool valid = next_valid;
-    const int key0 = range.tile(t) << L::kShift;
-    if (valid) {
+    // No key of a page outside the pool is seen: its tile lies behind every row.
+    const int key0 = next_there ? range.tile(t) << L::kShift : 1 << 30;
 #pragma unroll
-      for (int i = 0; i < L::kLoads; ++i) {
-        *reinterpret_cast<u32x4*>(kt + (k_to ^ L::k_turn(i * L::kStep)) + i * L::kStep * L::kBytes) = kst[i];
-        *reinterpret_cast<u32x4*>(vt + v_to + i * L::kStep * L::kBytes) = vst[i];
-      }
+    for (int i = 0; i < L::kLoads; ++i) {
+      *reinterpret_cast<u32x4*>(kt + (k_to ^ L::k_turn(i * L::kStep)) + i * L::kStep * L::kBytes) = kst[i];
+      *reinterpret_cast<u32x4*>(vt + v_to + i * L::kStep * L::kBytes) = vst[i];
     }
     // One barrier a tile: a wave past it has done with the other buffer, too.
     __syncthreads();
-    if (t + 1 < t_end) load(t + 1);
-    if (!valid || !wave_rows) continue;
-    if (key0 >= last.end || (key0 + L::kKeys <= first.low && key0 >= a.sinks)) continue;
+    load(t + 1);
     const bool whole = key0 + L::kKeys <= first.end && (key0 >= last.low || key0 + L::kKeys <= a.sinks);
 
     f32x16 sc[kKeyBlocks];
@@ -190,15 +189,19 @@ __global__ __launch_bounds__(kManyThreads, DP <= 128 ? 2 : 1) void attend_many_k
         sc[kb] = E::mfma32(kf, qf[st], sc[kb]);
       }
     }
+    if (!whole) {
+#pragma unroll
+      for (int kb = 0; kb < kKeyBlocks; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          sc[kb][i] = sees(sight, a.sinks, key0 + kb * 32 + 8 * (i >> 2) + 4 * half + (i & 3)) ? sc[kb][i] : kNegInf;
+    }
     float top = kNegInf;
 #pragma unroll
     for (int kb = 0; kb < kKeyBlocks; ++kb)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        if (!whole && !sees(sight, a.sinks, key0 + kb * 32 + 8 * (i >> 2) + 4 * half + (i & 3))) sc[kb][i] = kNegInf;
-        top = fmaxf(top, sc[kb][i]);
-      }
-    top = fmaxf(top, __shfl_xor(top, 32)) * a.scale_log2;
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[kb][i]);
+    top = max_across_halves(top) * a.scale_log2;
     // The maximum moves only when it grows by more than 2^8: weights then reach
     // 2^8 at most, and most tiles leave the outputs unscaled.
     const float m_new = top > m_run + 8.0f ? top : m_run;
