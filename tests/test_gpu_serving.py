@@ -406,6 +406,48 @@ def test_attend_more_requests_than_one_launch_takes(hip_device) -> None:
         torch.testing.assert_close(got[r : r + 1], one, rtol=2.0**-7, atol=2.0**-12)
 
 
+@pytest.mark.parametrize("n, longest, heads", [(70, 90, 8), (300, 40, 4), (5000, 12, 8)])
+def test_attend_chunks_of_many_requests(hip_device, n, longest, heads) -> None:
+    """Row tiles of more requests than a wave has lanes, between ones without any:
+    each request's rows are what it gets alone."""
+    g = torch.Generator(device=hip_device).manual_seed(n)
+    kv, dim = 2, 64
+    pool = torch.randn((2, 200, 128, kv, dim), generator=g, device=hip_device).to(BF16)
+    table = torch.randint(0, 200, (n, 3), generator=g, device=hip_device).int()
+    new = torch.randint(0, longest, (n,), generator=g, device=hip_device).int()
+    new[n // 3 : n // 2] = 0
+    new[[0, n // 2, n - 1]] = longest
+    lens = new + torch.randint(0, 250, (n,), generator=g, device=hip_device).int()
+    start = torch.cat([new.new_zeros(1), new.cumsum(0, dtype=torch.int32)])
+    host = start.tolist()
+    q = torch.randn((host[-1], heads, dim), generator=g, device=hip_device).to(BF16)
+    got = _serving().attend_paged(q, pool[0], pool[1], start, lens, table, max_query_len=longest)
+    assert torch.isfinite(got).all()
+    two = torch.empty(2, dtype=torch.int32, device=hip_device)
+    for r in sorted({0, 1, n // 3 - 1, n // 2, n // 2 + 1, 63 % n, 64, 65, n - 2, n - 1}):
+        size = host[r + 1] - host[r]
+        two[0], two[1] = 0, size
+        one = _serving().attend_paged(q[host[r] : host[r + 1]], pool[0], pool[1], two, lens[r : r + 1], table[r : r + 1])
+        torch.testing.assert_close(got[host[r] : host[r + 1]], one, rtol=2.0**-6, atol=2.0**-9)
+
+
+@pytest.mark.parametrize("tokens, total, kv, heads, window", [(900, 3000, 8, 40, 0), (700, 2500, 8, 40, 700), (1300, 1300, 2, 16, 0)])
+def test_attend_splits_what_whole_rounds_leave(hip_device, tokens, total, kv, heads, window) -> None:
+    """More (row tile, head) items than the device takes at once, or fewer: the ones left over are split."""
+    g = torch.Generator().manual_seed(tokens)
+    dim = 128
+    k, v, table = _paged([total], kv, dim, BF16, g)
+    q = torch.randn((tokens, heads, dim), generator=g).to(BF16)
+    d = lambda x: torch.tensor(x, dtype=torch.int32, device=hip_device)  # noqa: E731
+    got = _serving().attend_paged(q.to(hip_device), k.to(hip_device), v.to(hip_device), d([0, tokens]), d([total]), table.to(hip_device),
+                                  window=window, max_seq_len=total)
+    # Rows of the first, middle and last tiles, as requests of one token each.
+    picked = sorted({0, 1, 25, 26, 300, 301, tokens // 2, tokens - 27, tokens - 1})
+    lens = [total - tokens + i + 1 for i in picked]
+    _check(got[picked], q[picked], (k, v), list(range(len(picked) + 1)), lens, table.expand(len(picked), -1), BF16, scale=dim**-0.5,
+           window=window, sinks=0, rows_most=tokens)
+
+
 @pytest.mark.parametrize("new", [1, 40])
 def test_attend_under_capture_and_on_another_stream(hip_device, new) -> None:
     g = torch.Generator(device=hip_device).manual_seed(new)

@@ -13,8 +13,7 @@ constexpr int kCompute = 256;  // compute units of the device
 struct AttendPlan {
   int row_tiles;    // 16-row tiles a request of the few-rows kernel has at most; 0: kernel not needed
   int workgroups;   // of the few-rows kernel
-  int64_t tiles;    // 128-row tiles of the many-rows kernel; 0: kernel not needed
-  int splits;       // of their keys
+  ManyGrid many;    // of the many-rows kernel; no grid: kernel not needed
   int sequences;    // requests of one few-rows launch
   size_t bytes;     // workspace
 };
@@ -34,15 +33,17 @@ AttendPlan make_plan(int kv_heads, int qpk, int head_dim, int n_seq, int64_t num
     few = static_cast<size_t>(p.workgroups) * (16 + 8 * piece_floats(kFewRows * p.row_tiles, dim));
   }
   if (most_rows > kFewRows * p.row_tiles) {
-    p.tiles = num_tokens * qpk / kManyRows + n_seq;
-    // Two workgroups a compute unit are wanted; a split is not worth fewer than 512 keys.
-    const int64_t filled = ceil_div(num_tokens * qpk, kManyRows) * kv_heads;
-    int64_t splits = filled >= 2 * kCompute ? 1 : ceil_div(2 * kCompute, filled);
-    const int64_t by_keys = ceil_div(pages * kBlockSize, 512), by_space = 4096 / (p.tiles * kv_heads);
-    if (splits > by_keys) splits = by_keys;
-    if (splits > by_space) splits = by_space;
-    p.splits = splits < 1 ? 1 : static_cast<int>(splits);
-    if (p.splits > 1) many = static_cast<size_t>(p.tiles) * kv_heads * p.splits * piece_floats(kManyRows, dim) * 4;
+    // Row tiles are at most as many as all rows fill, and a partly filled one more
+    // for each request that has more rows than the few-rows kernel takes; one
+    // round more of workgroups is there for the items that are split, into no
+    // fewer than 512 keys.
+    const int64_t rows = num_tokens * qpk, most = rows / (kFewRows * p.row_tiles + 1);
+    const int64_t tiles = rows / kManyRows + (most < n_seq ? most : n_seq);
+    p.many.round = kCompute * many_residents(dim);
+    p.many.grid = tiles * kv_heads + p.many.round;
+    const int64_t by_keys = pages * kBlockSize / 512;
+    p.many.most_splits = static_cast<int>(by_keys < 1 ? 1 : (by_keys > p.many.round ? p.many.round : by_keys));
+    if (p.many.most_splits > 1) many = static_cast<size_t>(p.many.round) * piece_floats(kManyRows, dim) * 4;
   }
   p.bytes = few > many ? few : many;
   if (p.bytes == 0) p.bytes = 16;
@@ -93,7 +94,7 @@ extern "C" int kvc_attend_paged(kvc_stream_t stream, int dtype, const void* q, i
   const AttendPlan plan = make_plan(kv_heads, qpk, head_dim, n_seq, num_tokens, max_query_len, max_seq_len);
   if (!workspace || workspace_bytes < plan.bytes)
     return fail(KVC_EINVAL, "kvc_attend_paged: workspace too small (%zu of %zu bytes)", workspace_bytes, plan.bytes);
-  if (plan.tiles * kv_heads * plan.splits >= (1ll << 31))
+  if (plan.many.grid >= (1ll << 31))
     return fail(KVC_EINVAL, "kvc_attend_paged: too many rows for one launch");
 
   AttendArgs a = {};
@@ -135,13 +136,18 @@ extern "C" int kvc_attend_paged(kvc_stream_t stream, int dtype, const void* q, i
       if (int rc = launch_attend_few(st, f16, a, plan.workgroups, plan.row_tiles)) return rc;
     }
   }
-  if (plan.tiles) {
+  if (plan.many.grid) {
     a.n_seq = n_seq;
     a.start = query_start_loc;
     a.seq_lens = seq_lens;
     a.table = block_table;
     a.partial = static_cast<float*>(workspace);
-    if (int rc = launch_attend_many(st, f16, a, plan.tiles, plan.splits)) return rc;
+    ManyGrid grid = plan.many;
+    if (a.window) {  // a row tile's keys are fewer than the request's
+      const int64_t most = (static_cast<int64_t>(a.window) + sinks + kManyRows) / 512;
+      if (most < grid.most_splits) grid.most_splits = most < 1 ? 1 : static_cast<int>(most);
+    }
+    if (int rc = launch_attend_many(st, f16, a, grid)) return rc;
   }
   return 0;
 }

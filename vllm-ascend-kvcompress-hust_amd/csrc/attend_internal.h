@@ -219,9 +219,16 @@ __device__ __forceinline__ void join_pieces(int count, int first, int rows, int 
   if (working && share == 0) store(row, d, sum);
 }
 
+// The many-rows launch: `round` workgroups fit the device at once, `grid` are
+// launched, and a (row tile, head)'s keys are split at most `most_splits` times.
+struct ManyGrid {
+  int round, most_splits;
+  int64_t grid;
+};
+
 // Entry points of the kernels' files.
 int launch_attend_few(hipStream_t stream, bool f16, const AttendArgs& a, int workgroups, int row_tiles);
-int launch_attend_many(hipStream_t stream, bool f16, const AttendArgs& a, int64_t tiles, int splits);
+int launch_attend_many(hipStream_t stream, bool f16, const AttendArgs& a, const ManyGrid& grid);
 
 // Sizes of the workspace's parts.
 constexpr int kFewRows = 16;         // rows of one few-rows tile
@@ -231,6 +238,9 @@ constexpr int kManyRows = 128;       // rows of one many-rows tile
 
 // Few-rows workgroups that a compute unit holds.
 constexpr int few_residents(int dim, int row_tiles) { return dim <= 64 ? 4 - row_tiles : (dim <= 128 ? 2 : 1); }
+
+// Many-rows workgroups that a compute unit holds.
+constexpr int many_residents(int dim) { return dim <= 128 ? 2 : 1; }
 
 // Floats of a piece of `rows` rows: unnormalised outputs, then (max, sum) pairs.
 __host__ __device__ inline int64_t piece_floats(int rows, int dim) { return static_cast<int64_t>(rows) * (dim + 2); }

@@ -41,33 +41,83 @@ struct ManyLayout {
   __device__ __forceinline__ static constexpr int v_turn(int row) { return (kRow == 64 ? (row >> 1) & 1 : row & 3) << 6; }
 };
 
-// The row tile and request of a workgroup: request r owns tiles from
-// start[r]*qpk/128 + r, which leaves room for its last, partly filled one.
-struct ManyTile {
-  int request, row0;
+// Row tiles of request r that are this kernel's.
+__device__ __forceinline__ int tiles_of(const AttendArgs& a, int r) {
+  const int64_t total = a.num_tokens;
+  int64_t t0 = a.start[r], t1 = a.start[r + 1];
+  t0 = t0 < 0 ? 0 : (t0 > total ? total : t0);
+  t1 = t1 < t0 ? t0 : (t1 > total ? total : t1);
+  const int64_t rows = (t1 - t0) * a.qpk;
+  return rows > a.few_rows ? static_cast<int>((rows + kManyRows - 1) / kManyRows) : 0;
+}
+
+__device__ __forceinline__ int sum_up_to_lane(int x) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int up = __shfl_up(x, d);
+    if (lane >= d) x += up;
+  }
+  return x;
+}
+
+// Row tiles of all requests, counted by one wave: a lane sums its share of them.
+struct TileCount {
+  int share, sum;  // requests a lane, tiles up to the end of the lane's
+  __device__ __forceinline__ TileCount(const AttendArgs& a) {
+    const int lane = threadIdx.x & 63;
+    share = (a.n_seq + 63) / 64;
+    int mine = 0;
+    for (int i = 0; i < share; ++i) {
+      const int r = lane * share + i;
+      if (r < a.n_seq) mine += tiles_of(a, r);
+    }
+    sum = sum_up_to_lane(mine);
+  }
+  __device__ __forceinline__ int total() const { return __builtin_amdgcn_readlane(sum, 63); }
+  // The request of row tile `tile` < total(), and the tile's number in it.
+  __device__ __forceinline__ void find(const AttendArgs& a, int tile, int* request, int* local) const {
+    const int at = __builtin_ctzll(__ballot(sum > tile));  // the first lane whose share ends behind it
+    int before = at ? __builtin_amdgcn_readlane(sum, at > 0 ? at - 1 : 0) : 0;
+    for (int base = at * share;; base += 64) {
+      const int r = base + static_cast<int>(threadIdx.x & 63);
+      const int up = sum_up_to_lane(r < a.n_seq && r < (at + 1) * share ? tiles_of(a, r) : 0);
+      const uint64_t behind = __ballot(before + up > tile);
+      if (behind || base + 64 >= (at + 1) * share) {
+        const int in = behind ? __builtin_ctzll(behind) : 0;
+        *request = base + in;
+        *local = tile - before - (in ? __builtin_amdgcn_readlane(up, in > 0 ? in - 1 : 0) : 0);
+        return;
+      }
+      before += __builtin_amdgcn_readlane(up, 63);
+    }
+  }
 };
 
-__device__ __forceinline__ int64_t tile_base(const AttendArgs& a, int r) {
-  int64_t t = scalar_at(a.start, r);
-  t = t < 0 ? 0 : (t > a.num_tokens ? a.num_tokens : t);
-  return t * a.qpk / kManyRows + r;
-}
-
-__device__ __forceinline__ ManyTile tile_of(const AttendArgs& a, int64_t tile) {
-  int low = 0, high = a.n_seq;  // base(low) <= tile < base(high)
-  while (high - low > 1) {
-    const int mid = (low + high) >> 1;
-    if (tile_base(a, mid) <= tile)
-      low = mid;
+// How the (row tile, head) items are shared out: whole rounds of the device take
+// one item a workgroup; what is left over (or all, where there is no whole
+// round) is split along its keys into one more round.  From six rounds on, the
+// last, partly filled one is a small share and nothing is split.
+constexpr int kManyRounds = 6;
+struct ManyShares {
+  int total, whole, splits;  // row tiles; those (the last ones) that are not split
+  __device__ __forceinline__ ManyShares(const AttendArgs& a, const ManyGrid& grid, int tiles) : total(tiles), whole(tiles), splits(1) {
+    const int64_t items = static_cast<int64_t>(tiles) * a.kv_heads;
+    const int rounds = static_cast<int>(items / grid.round < kManyRounds ? items / grid.round : kManyRounds);
+    if (rounds >= kManyRounds) return;
+    const int left = tiles - static_cast<int>(static_cast<int64_t>(rounds) * grid.round / a.kv_heads);
+    if (left <= 0) return;
+    const int fit = static_cast<int>(grid.round / (static_cast<int64_t>(left) * a.kv_heads));
+    splits = fit < grid.most_splits ? fit : grid.most_splits;
+    if (splits > 1)
+      whole = tiles - left;
     else
-      high = mid;
+      splits = 1;
   }
-  const int64_t row0 = (tile - tile_base(a, low)) * kManyRows;
-  return {low, row0 < 0 || row0 > 0x7fffff00 ? 0x7fffff00 : static_cast<int>(row0)};
-}
+};
 
 template <bool F16, int DP>
-__global__ __launch_bounds__(kManyThreads, DP <= 128 ? 2 : 1) void attend_many_kernel(AttendArgs a, int64_t tiles, int splits) {
+__global__ __launch_bounds__(kManyThreads, many_residents(DP)) void attend_many_kernel(AttendArgs a, ManyGrid grid) {
   typedef AttendElem<F16> E;
   typedef typename E::vec vec_t;
   typedef ManyLayout<DP> L;
@@ -77,32 +127,39 @@ __global__ __launch_bounds__(kManyThreads, DP <= 128 ? 2 : 1) void attend_many_k
   __shared__ __attribute__((aligned(16))) uint16_t k_tile[2][L::kTile];
   __shared__ __attribute__((aligned(16))) uint16_t v_tile[2][L::kTile];
 
+  // The last rows see the most keys: they begin first, and the ones that are
+  // split end last.
   const int head = blockIdx.x % a.kv_heads;
-  const int rest = blockIdx.x / a.kv_heads;
-  const int split = rest % splits;
-  const int64_t tile = tiles - 1 - rest / splits;  // the last rows see the most keys: they begin first
-  const ManyTile mine = tile_of(a, tile);
-  const Request s = uniform_request_of(a, mine.request);
-  const int64_t all_rows = static_cast<int64_t>(s.fresh) * a.qpk;
-  if (mine.row0 >= all_rows || all_rows <= a.few_rows) return;
-  const int rows = static_cast<int>(all_rows);
+  const int order = blockIdx.x / a.kv_heads;
+  const TileCount counted(a);
+  const ManyShares shares(a, grid, counted.total());
+  const bool divided = order >= shares.whole;
+  const int splits = divided ? shares.splits : 1;
+  const int split = divided ? (order - shares.whole) % splits : 0;
+  const int item = divided ? (order - shares.whole) / splits : 0;  // of the split ones
+  const int tile = shares.total - 1 - (divided ? shares.whole + item : order);
+  if (tile < 0) return;
+  int request, local;
+  counted.find(a, tile, &request, &local);
+  const Request s = uniform_request_of(a, request);
+  const int rows = s.fresh * a.qpk, row0 = local * kManyRows;
 
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
   const int wave = uniform(tid >> 6);
   const int place0 = s.len - s.fresh;
-  const int wg_last = (mine.row0 + kManyRows < rows ? mine.row0 + kManyRows : rows) - 1;
-  const TileRange range = tile_range<L::kShift>(a, s, place0 + mine.row0 / a.qpk, place0 + wg_last / a.qpk);
+  const int wg_last = (row0 + kManyRows < rows ? row0 + kManyRows : rows) - 1;
+  const TileRange range = tile_range<L::kShift>(a, s, place0 + row0 / a.qpk, place0 + wg_last / a.qpk);
   const int count = range.count();
   const int t_begin = static_cast<int>(static_cast<int64_t>(count) * split / splits);
   const int t_end = static_cast<int>(static_cast<int64_t>(count) * (split + 1) / splits);
 
-  const int m = mine.row0 + wave * 32 + col;
+  const int m = row0 + wave * 32 + col;
   const bool inside = m < rows;
   const int token = (inside ? m : rows - 1) / a.qpk, g = (inside ? m : rows - 1) - token * a.qpk;
   RowSight sight = sight_of(a, s, place0 + token);
   if (!inside) sight.end = 0;
   // The wave's first and last rows' sights.
-  const int m_first = mine.row0 + wave * 32, m_last = m_first + 31 < rows ? m_first + 31 : rows - 1;
+  const int m_first = row0 + wave * 32, m_last = m_first + 31 < rows ? m_first + 31 : rows - 1;
   const int token_first = m_first / a.qpk, token_last = (m_first < rows ? m_last : m_first) / a.qpk;
   const RowSight first = sight_of(a, s, place0 + token_first), last = sight_of(a, s, place0 + token_last);
 
@@ -119,7 +176,7 @@ __global__ __launch_bounds__(kManyThreads, DP <= 128 ? 2 : 1) void attend_many_k
   }
   const int row_elems = a.kv_heads * a.head_dim;
   const uint32_t row_bytes = row_elems * 2;
-  const int32_t* table = a.table + mine.request * a.table_stride;
+  const int32_t* table = a.table + request * a.table_stride;
   // The thread's chunk of a tile's first rows: where it is (behind everything
   // where the row has none) and where it goes, then where the lane reads.
   const int row_to = tid / L::kSlots, chunk_to = tid & (L::kSlots - 1);
@@ -281,7 +338,7 @@ __global__ __launch_bounds__(kManyThreads, DP <= 128 ? 2 : 1) void attend_many_k
 
   const float l_all = l_run + __shfl_xor(l_run, 32);
   if (!inside) return;
-  if (splits == 1) {
+  if (!divided) {
     const float inv = l_all == 0.0f ? 0.0f : 1.0f / l_all;
     uint16_t* to = a.out + (s.token0 + token) * a.out_token_stride + (head * a.qpk + g) * a.out_head_stride;
 #pragma unroll
@@ -294,8 +351,8 @@ __global__ __launch_bounds__(kManyThreads, DP <= 128 ? 2 : 1) void attend_many_k
               u32x2{E::pack(acc[b][4 * i] * inv, acc[b][4 * i + 1] * inv), E::pack(acc[b][4 * i + 2] * inv, acc[b][4 * i + 3] * inv)};
       }
   } else {
-    float* const piece = a.partial + ((tile * a.kv_heads + head) * splits + split) * piece_floats(kManyRows, DP);
-    const int local = m - mine.row0;
+    float* const piece = a.partial + ((static_cast<int64_t>(item) * a.kv_heads + head) * splits + split) * piece_floats(kManyRows, DP);
+    const int local = m - row0;
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
@@ -306,54 +363,59 @@ __global__ __launch_bounds__(kManyThreads, DP <= 128 ? 2 : 1) void attend_many_k
   }
 }
 
-// Joins the splits of a (row tile, KV head), four rows a workgroup.
+// Joins the splits of a (row tile, KV head), 16 rows a workgroup, four at a time.
 template <bool F16, int DP>
-__global__ __launch_bounds__(kManyThreads) void attend_many_join_kernel(AttendArgs a, int splits) {
+__global__ __launch_bounds__(kManyThreads) void attend_many_join_kernel(AttendArgs a, ManyGrid grid) {
   typedef AttendElem<F16> E;
-  const int head = blockIdx.x % a.kv_heads, row0 = blockIdx.y * 4;
-  const int64_t tile = blockIdx.x / a.kv_heads;
-  const ManyTile mine = tile_of(a, tile);
-  const Request s = uniform_request_of(a, mine.request);
-  const int64_t all_rows = static_cast<int64_t>(s.fresh) * a.qpk;
-  if (mine.row0 + row0 >= all_rows || all_rows <= a.few_rows) return;
-  const int rows = all_rows - mine.row0 < kManyRows ? static_cast<int>(all_rows - mine.row0) : kManyRows;
+  const int head = blockIdx.x % a.kv_heads, item = blockIdx.x / a.kv_heads;
+  const TileCount counted(a);
+  const ManyShares shares(a, grid, counted.total());
+  const int tile = shares.total - 1 - shares.whole - item;
+  if (tile < 0) return;
+  int request, local_tile;
+  counted.find(a, tile, &request, &local_tile);
+  const Request s = uniform_request_of(a, request);
+  const int row0 = local_tile * kManyRows, left = s.fresh * a.qpk - row0;
   const int64_t size = piece_floats(kManyRows, DP);
-  const float* const pieces = a.partial + (tile * a.kv_heads + head) * splits * size;
-  join_pieces<DP>(
-      splits, row0, rows, a.head_dim, kManyRows * DP, [&](int i) { return pieces + i * size; },
-      [&](int local, int d, f32x4 x) {
-        const int m = mine.row0 + local, token = m / a.qpk, g = m - token * a.qpk;
-        uint16_t* to = a.out + (s.token0 + token) * a.out_token_stride + (head * a.qpk + g) * a.out_head_stride;
-        *gptr(reinterpret_cast<u32x2*>(to + d)) = u32x2{E::pack(x[0], x[1]), E::pack(x[2], x[3])};
-      });
+  const float* const pieces = a.partial + (static_cast<int64_t>(item) * a.kv_heads + head) * shares.splits * size;
+  const int begin = blockIdx.y * 16, end = left < begin + 16 ? left : begin + 16;
+  for (int row = begin; row < end; row += 4) {
+    if (row > begin) __syncthreads();
+    join_pieces<DP>(
+        shares.splits, row, end, a.head_dim, kManyRows * DP, [&](int i) { return pieces + i * size; },
+        [&](int local, int d, f32x4 x) {
+          const int m = row0 + local, token = m / a.qpk, g = m - token * a.qpk;
+          uint16_t* to = a.out + (s.token0 + token) * a.out_token_stride + (head * a.qpk + g) * a.out_head_stride;
+          *gptr(reinterpret_cast<u32x2*>(to + d)) = u32x2{E::pack(x[0], x[1]), E::pack(x[2], x[3])};
+        });
+  }
 }
 
 template <bool F16, int DP>
-int launch(hipStream_t stream, const AttendArgs& a, int64_t tiles, int splits) {
-  attend_many_kernel<F16, DP>
-      <<<static_cast<unsigned>(tiles * a.kv_heads * splits), kManyThreads, 0, stream>>>(a, tiles, splits);
+int launch(hipStream_t stream, const AttendArgs& a, const ManyGrid& grid) {
+  attend_many_kernel<F16, DP><<<static_cast<unsigned>(grid.grid), kManyThreads, 0, stream>>>(a, grid);
   if (int rc = launch_status("kvc_attend_paged")) return rc;
-  if (splits > 1)
-    attend_many_join_kernel<F16, DP>
-        <<<dim3(static_cast<unsigned>(tiles * a.kv_heads), kManyRows / 4), kManyThreads, 0, stream>>>(a, splits);
+  // Split items number half a round at most: each has two splits or more.
+  if (grid.most_splits > 1)
+    attend_many_join_kernel<F16, DP><<<dim3(grid.round / 2, kManyRows / 16), kManyThreads, 0, stream>>>(a, grid);
   return launch_status("kvc_attend_paged");
 }
 
 template <bool F16>
-int pick_dim(hipStream_t stream, const AttendArgs& a, int64_t tiles, int splits) {
+int pick_dim(hipStream_t stream, const AttendArgs& a, const ManyGrid& grid) {
   switch (padded_dim(a.head_dim)) {
-    case 64: return launch<F16, 64>(stream, a, tiles, splits);
-    case 96: return launch<F16, 96>(stream, a, tiles, splits);
-    case 128: return launch<F16, 128>(stream, a, tiles, splits);
-    case 192: return launch<F16, 192>(stream, a, tiles, splits);
-    default: return launch<F16, 256>(stream, a, tiles, splits);
+    case 64: return launch<F16, 64>(stream, a, grid);
+    case 96: return launch<F16, 96>(stream, a, grid);
+    case 128: return launch<F16, 128>(stream, a, grid);
+    case 192: return launch<F16, 192>(stream, a, grid);
+    default: return launch<F16, 256>(stream, a, grid);
   }
 }
 
 }  // namespace
 
-int launch_attend_many(hipStream_t stream, bool f16, const AttendArgs& a, int64_t tiles, int splits) {
-  return f16 ? pick_dim<true>(stream, a, tiles, splits) : pick_dim<false>(stream, a, tiles, splits);
+int launch_attend_many(hipStream_t stream, bool f16, const AttendArgs& a, const ManyGrid& grid) {
+  return f16 ? pick_dim<true>(stream, a, grid) : pick_dim<false>(stream, a, grid);
 }
 
 }  // namespace kvc
