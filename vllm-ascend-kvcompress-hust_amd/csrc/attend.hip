@@ -24,7 +24,10 @@ AttendPlan make_plan(int kv_heads, int qpk, int head_dim, int n_seq, int64_t num
   const int64_t most_rows = static_cast<int64_t>(max_query_len) * qpk;
   const int64_t pages = ceil_div(max_seq_len > 0 ? max_seq_len : 1, kBlockSize);
   size_t few = 0, many = 0;
-  if (qpk <= kFewRows * kFewTilesMost) {
+  // A lone request of many rows leaves the few-rows kernel nothing; whatever its
+  // real length, the many-rows kernel takes it.
+  const bool lone = n_seq == 1 && most_rows > kFewRows * kFewTilesMost;
+  if (qpk <= kFewRows * kFewTilesMost && !lone) {
     p.row_tiles = most_rows <= kFewRows ? 1 : kFewTilesMost;
     p.sequences = n_seq < kFewSequences ? n_seq : kFewSequences;
     const int64_t bound = static_cast<int64_t>(p.sequences) * kv_heads * pages;
@@ -38,12 +41,12 @@ AttendPlan make_plan(int kv_heads, int qpk, int head_dim, int n_seq, int64_t num
     // round more of workgroups is there for the items that are split, into no
     // fewer than 512 keys.
     const int64_t rows = num_tokens * qpk, most = rows / (kFewRows * p.row_tiles + 1);
-    const int64_t tiles = rows / kManyRows + (most < n_seq ? most : n_seq);
-    p.many.round = kCompute * many_residents(dim);
+    const int64_t tiles = rows / many_rows(dim) + (most < n_seq ? most : n_seq);
+    p.many.round = kCompute;  // one workgroup a compute unit
     p.many.grid = tiles * kv_heads + p.many.round;
     const int64_t by_keys = pages * kBlockSize / 512;
     p.many.most_splits = static_cast<int>(by_keys < 1 ? 1 : (by_keys > p.many.round ? p.many.round : by_keys));
-    if (p.many.most_splits > 1) many = static_cast<size_t>(p.many.round) * piece_floats(kManyRows, dim) * 4;
+    if (p.many.most_splits > 1) many = static_cast<size_t>(p.many.round) * piece_floats(many_rows(dim), dim) * 4;
   }
   p.bytes = few > many ? few : many;
   if (p.bytes == 0) p.bytes = 16;
@@ -78,8 +81,9 @@ extern "C" int kvc_attend_paged(kvc_stream_t stream, int dtype, const void* q, i
                 "kvc_attend_paged: bad sizes (head_dim %d must be a multiple of 8 up to 256; kv_heads %d, qpk %d at most 1024; "
                 "n_seq %d, num_tokens %lld below 2^24)",
                 head_dim, kv_heads, qpk, n_seq, static_cast<long long>(num_tokens));
-  if (num_pages < 0 || page_stride < static_cast<int64_t>(kBlockSize) * kv_heads * head_dim || page_stride % 8)
-    return fail(KVC_EINVAL, "kvc_attend_paged: page_stride must be a multiple of 8 elements and at least one page");
+  if (num_pages < 0 || page_stride < static_cast<int64_t>(kBlockSize) * kv_heads * head_dim || page_stride % 8 ||
+      page_stride >= (1ll << 31))
+    return fail(KVC_EINVAL, "kvc_attend_paged: page_stride must be a multiple of 8 elements, at least one page and below 2^31");
   if (max_blocks < 0 || max_blocks >= (1 << 23) || block_table_stride < max_blocks)
     return fail(KVC_EINVAL, "kvc_attend_paged: max_blocks must be below 2^23 and at most block_table_stride");
   if (!(scale > 0.0f) || !isfinite(scale)) return fail(KVC_EINVAL, "kvc_attend_paged: scale must be positive and finite");
@@ -106,8 +110,8 @@ extern "C" int kvc_attend_paged(kvc_stream_t stream, int dtype, const void* q, i
   a.q_head_stride = q_head_stride;
   a.out_token_stride = out_token_stride;
   a.out_head_stride = out_head_stride;
-  a.num_pages = num_pages;
-  a.page_stride = page_stride;
+  a.num_pages = num_pages < 0x7fffffff ? static_cast<int>(num_pages) : 0x7fffffff;
+  a.page_bytes = static_cast<uint32_t>(page_stride * 2);
   a.table_stride = block_table_stride;
   a.num_tokens = num_tokens;
   a.scale_log2 = scale * 1.4426950408889634f;
@@ -144,7 +148,7 @@ extern "C" int kvc_attend_paged(kvc_stream_t stream, int dtype, const void* q, i
     a.partial = static_cast<float*>(workspace);
     ManyGrid grid = plan.many;
     if (a.window) {  // a row tile's keys are fewer than the request's
-      const int64_t most = (static_cast<int64_t>(a.window) + sinks + kManyRows) / 512;
+      const int64_t most = (static_cast<int64_t>(a.window) + sinks + many_rows(padded_dim(head_dim))) / 512;
       if (most < grid.most_splits) grid.most_splits = most < 1 ? 1 : static_cast<int>(most);
     }
     if (int rc = launch_attend_many(st, f16, a, grid)) return rc;

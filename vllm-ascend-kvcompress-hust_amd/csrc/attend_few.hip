@@ -165,7 +165,7 @@ __global__ __launch_bounds__(kFewThreads, few_residents(DP, NQ)) void attend_few
     // page is in the pool.
     struct Slice {
       int tile, key0;
-      int64_t base;
+      uint64_t base;  // bytes
     };
     const int32_t* const table = a.table + r * a.table_stride;
     PageIds ids;
@@ -178,7 +178,7 @@ __global__ __launch_bounds__(kFewThreads, few_residents(DP, NQ)) void attend_few
         if (f.key0 >= last_end || (f.key0 + kSliceKeys <= first_low && f.key0 >= a.sinks)) continue;
         const int page = ids.at(table, a.max_blocks, block);
         if (page < 0 || page >= a.num_pages) continue;
-        f.base = page * a.page_stride + static_cast<int64_t>(wave * kSliceKeys) * row_elems + head * a.head_dim;
+        f.base = static_cast<uint64_t>(static_cast<uint32_t>(page)) * a.page_bytes + wave * kSliceKeys * row_bytes + head * a.head_dim * 2;
         break;
       }
       return f;
@@ -187,7 +187,7 @@ __global__ __launch_bounds__(kFewThreads, few_residents(DP, NQ)) void attend_few
     // page (K) or the request's last row (V: whatever the page holds there).
     u32x4 kw[2][kSteps], vw[Layout::kLoads];
     auto load_k = [&](const Slice& f) {
-      const auto from = page_rsrc(a.k + f.base, kSliceKeys * row_bytes - head * a.head_dim * 2);
+      const auto from = page_rsrc(a.k, f.base, kSliceKeys * row_bytes - head * a.head_dim * 2);
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -196,7 +196,7 @@ __global__ __launch_bounds__(kFewThreads, few_residents(DP, NQ)) void attend_few
     };
     auto load_v = [&](const Slice& f) {
       const int left = s.keys - f.key0 < kSliceKeys ? s.keys - f.key0 : kSliceKeys;
-      const auto from = page_rsrc(a.v + f.base, (left - 1) * row_bytes + a.head_dim * 2);
+      const auto from = page_rsrc(a.v, f.base, (left - 1) * row_bytes + a.head_dim * 2);
 #pragma unroll
       for (int i = 0; i < Layout::kLoads; ++i)
         vw[i] = __builtin_amdgcn_raw_buffer_load_b128(from, v_lane, i * Layout::kStep * row_bytes, kNonTemporal);

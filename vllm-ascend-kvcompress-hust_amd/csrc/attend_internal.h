@@ -32,7 +32,9 @@ struct AttendArgs {
   float* partial;           // joined pieces, see the kernels
   int32_t* header;
   int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
-  int64_t num_pages, page_stride, table_stride, num_tokens;
+  int64_t table_stride, num_tokens;
+  uint32_t page_bytes;  // from a page to the next
+  int num_pages;
   float scale_log2;  // scale * log2(e): weights are powers of two
   int n_seq, kv_heads, qpk, head_dim, max_blocks, window, sinks;
   int few_rows;  // requests of at most this many rows are the few-rows kernel's
@@ -152,15 +154,35 @@ struct PageIds {
   }
 };
 
+// The same for a walk in order, as places: a lane holds its page's first byte in
+// a pool, and whether the page is in it.
+struct PagePlaces {
+  int first = -(1 << 30);  // nothing yet
+  uint32_t low = 0, high = 0, there = 0;
+  __device__ __forceinline__ bool covers(int block) const { return static_cast<uint32_t>(block - first) < 64u; }
+  __device__ __forceinline__ void refill(const AttendArgs& a, const int32_t* table, int block) {
+    first = block;
+    const int mine = block + static_cast<int>(threadIdx.x & 63);
+    const int page = mine < a.max_blocks ? *gptr(table + mine) : -1;
+    const bool in = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.num_pages);
+    const uint64_t from = in ? static_cast<uint64_t>(static_cast<uint32_t>(page)) * a.page_bytes : 0;
+    low = static_cast<uint32_t>(from);
+    high = static_cast<uint32_t>(from >> 32);
+    there = in ? 0xffffffffu : 0;
+    asm volatile("" : "+v"(low), "+v"(high), "+v"(there));  // waited for here, not wherever they are used
+  }
+};
+
 // The larger of a lane's value and that of the lane 32 away.
 __device__ __forceinline__ float max_across_halves(float x) {
   const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
 }
 
-// A buffer of `bytes` bytes for loads with lane offsets; past its end they give zeros.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t page_rsrc(const uint16_t* base, uint32_t bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, bytes, 0x00020000);
+// A buffer of `bytes` bytes, `from` bytes behind a pool's start, for loads with
+// lane offsets; past its end they give zeros.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t page_rsrc(const uint16_t* pool, uint64_t from, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)(reinterpret_cast<uintptr_t>(pool) + from), 0, bytes, 0x00020000);
 }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -234,13 +256,11 @@ int launch_attend_many(hipStream_t stream, bool f16, const AttendArgs& a, const 
 constexpr int kFewRows = 16;         // rows of one few-rows tile
 constexpr int kFewTilesMost = 2;     // tiles of a request that the few-rows kernel takes
 constexpr int kFewSequences = 1024;  // requests of one launch (their prefix sums sit in LDS)
-constexpr int kManyRows = 128;       // rows of one many-rows tile
+// Rows of one many-rows tile, 32 a wave.
+constexpr int many_rows(int dim) { return dim <= 128 ? 256 : 128; }
 
 // Few-rows workgroups that a compute unit holds.
 constexpr int few_residents(int dim, int row_tiles) { return dim <= 64 ? 4 - row_tiles : (dim <= 128 ? 2 : 1); }
-
-// Many-rows workgroups that a compute unit holds.
-constexpr int many_residents(int dim) { return dim <= 128 ? 2 : 1; }
 
 // Floats of a piece of `rows` rows: unnormalised outputs, then (max, sum) pairs.
 __host__ __device__ inline int64_t piece_floats(int rows, int dim) { return static_cast<int64_t>(rows) * (dim + 2); }

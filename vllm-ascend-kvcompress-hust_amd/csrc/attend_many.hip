@@ -14,13 +14,27 @@
 // maxima, sums and outputs stay in float32.
 
 #include <type_traits>
+#include <utility>
 
 #include "attend_internal.h"
 
 namespace kvc {
 namespace {
 
-constexpr int kManyThreads = 256;
+#define KVC_INLINE __attribute__((always_inline))
+
+// f(FROM), f(FROM + 1), .. f(TO - 1) with constant numbers, whatever the compiler
+// thinks of unrolling.
+template <int FROM, typename F, int... I>
+__device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F f) {
+  (f(std::integral_constant<int, FROM + I>{}), ...);
+}
+template <int FROM, int TO, typename F>
+__device__ __forceinline__ void each(F f) {
+  each_of<FROM>(std::make_integer_sequence<int, TO - FROM>{}, f);
+}
+
+constexpr int kJoinThreads = 256;
 
 // K's and V's place in LDS: rows of 64, 128 or 256 elements whose 16-byte chunks
 // are moved, by an exclusive or with a number of the row, so that the 16 rows of
@@ -35,20 +49,23 @@ struct ManyLayout {
   static constexpr int kBytes = kRow * 2;
   static constexpr int kTile = kKeys * kRow;
   static constexpr int kSlots = kRow / 8;
-  static constexpr int kStep = kManyThreads / kSlots;
+  static constexpr int kGroups = many_rows(DP) / 128;  // of four waves, 32 rows each
+  static constexpr int kThreads = 256 * kGroups;
+  static constexpr int kStep = kThreads / kSlots;
   static constexpr int kLoads = kKeys / kStep;
   __device__ __forceinline__ static constexpr int k_turn(int row) { return (kRow == 64 ? (row >> 1) & 7 : row & 15) << 4; }
   __device__ __forceinline__ static constexpr int v_turn(int row) { return (kRow == 64 ? (row >> 1) & 1 : row & 3) << 6; }
 };
 
 // Row tiles of request r that are this kernel's.
+template <int ROWS>
 __device__ __forceinline__ int tiles_of(const AttendArgs& a, int r) {
   const int64_t total = a.num_tokens;
   int64_t t0 = a.start[r], t1 = a.start[r + 1];
   t0 = t0 < 0 ? 0 : (t0 > total ? total : t0);
   t1 = t1 < t0 ? t0 : (t1 > total ? total : t1);
   const int64_t rows = (t1 - t0) * a.qpk;
-  return rows > a.few_rows ? static_cast<int>((rows + kManyRows - 1) / kManyRows) : 0;
+  return rows > a.few_rows ? static_cast<int>((rows + ROWS - 1) / ROWS) : 0;
 }
 
 __device__ __forceinline__ int sum_up_to_lane(int x) {
@@ -62,6 +79,7 @@ __device__ __forceinline__ int sum_up_to_lane(int x) {
 }
 
 // Row tiles of all requests, counted by one wave: a lane sums its share of them.
+template <int ROWS>
 struct TileCount {
   int share, sum;  // requests a lane, tiles up to the end of the lane's
   __device__ __forceinline__ TileCount(const AttendArgs& a) {
@@ -70,7 +88,7 @@ struct TileCount {
     int mine = 0;
     for (int i = 0; i < share; ++i) {
       const int r = lane * share + i;
-      if (r < a.n_seq) mine += tiles_of(a, r);
+      if (r < a.n_seq) mine += tiles_of<ROWS>(a, r);
     }
     sum = sum_up_to_lane(mine);
   }
@@ -81,7 +99,7 @@ struct TileCount {
     int before = at ? __builtin_amdgcn_readlane(sum, at > 0 ? at - 1 : 0) : 0;
     for (int base = at * share;; base += 64) {
       const int r = base + static_cast<int>(threadIdx.x & 63);
-      const int up = sum_up_to_lane(r < a.n_seq && r < (at + 1) * share ? tiles_of(a, r) : 0);
+      const int up = sum_up_to_lane(r < a.n_seq && r < (at + 1) * share ? tiles_of<ROWS>(a, r) : 0);
       const uint64_t behind = __ballot(before + up > tile);
       if (behind || base + 64 >= (at + 1) * share) {
         const int in = behind ? __builtin_ctzll(behind) : 0;
@@ -117,21 +135,22 @@ struct ManyShares {
 };
 
 template <bool F16, int DP>
-__global__ __launch_bounds__(kManyThreads, many_residents(DP)) void attend_many_kernel(AttendArgs a, ManyGrid grid) {
+__global__ __launch_bounds__(ManyLayout<DP>::kThreads, ManyLayout<DP>::kGroups) void attend_many_kernel(AttendArgs a, ManyGrid grid) {
   typedef AttendElem<F16> E;
   typedef typename E::vec vec_t;
   typedef ManyLayout<DP> L;
+  constexpr int kRows = many_rows(DP);
   constexpr int kSteps = DP / 16;       // 16-dim steps of K Q^T
   constexpr int kBlocks = DP / 32;      // 32-dim blocks of the output
   constexpr int kKeyBlocks = L::kKeys / 32;
-  __shared__ __attribute__((aligned(16))) uint16_t k_tile[2][L::kTile];
-  __shared__ __attribute__((aligned(16))) uint16_t v_tile[2][L::kTile];
+  __shared__ __attribute__((aligned(16))) uint16_t k_tile[3][L::kTile];
+  __shared__ __attribute__((aligned(16))) uint16_t v_tile[3][L::kTile];
 
   // The last rows see the most keys: they begin first, and the ones that are
   // split end last.
   const int head = blockIdx.x % a.kv_heads;
   const int order = blockIdx.x / a.kv_heads;
-  const TileCount counted(a);
+  const TileCount<kRows> counted(a);
   const ManyShares shares(a, grid, counted.total());
   const bool divided = order >= shares.whole;
   const int splits = divided ? shares.splits : 1;
@@ -142,12 +161,12 @@ __global__ __launch_bounds__(kManyThreads, many_residents(DP)) void attend_many_
   int request, local;
   counted.find(a, tile, &request, &local);
   const Request s = uniform_request_of(a, request);
-  const int rows = s.fresh * a.qpk, row0 = local * kManyRows;
+  const int rows = s.fresh * a.qpk, row0 = local * kRows;
 
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
   const int wave = uniform(tid >> 6);
   const int place0 = s.len - s.fresh;
-  const int wg_last = (row0 + kManyRows < rows ? row0 + kManyRows : rows) - 1;
+  const int wg_last = (row0 + kRows < rows ? row0 + kRows : rows) - 1;
   const TileRange range = tile_range<L::kShift>(a, s, place0 + row0 / a.qpk, place0 + wg_last / a.qpk);
   const int count = range.count();
   const int t_begin = static_cast<int>(static_cast<int64_t>(count) * split / splits);
@@ -190,75 +209,222 @@ __global__ __launch_bounds__(kManyThreads, many_residents(DP)) void attend_many_
   // The queries are there before the first tile is asked for: the loop's waits
   // then count its own loads alone.
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-  PageIds pages;
-  bool next_there = false;
-  // Zeros from behind the last tile, from pages outside the pool and from behind
-  // the request's last row, whatever the page holds there.
-  auto load = [&](int t) {
-    const int key0 = range.tile(t < t_end ? t : t_end - 1) << L::kShift;
-    const int page = pages.at(table, a.max_blocks, key0 >> kBlockShift);
-    next_there = (t < t_end) & (page >= 0) & (page < a.num_pages);
-    const int64_t base = (next_there ? page : 0) * a.page_stride + static_cast<int64_t>(key0 & (kBlockSize - 1)) * row_elems + head * a.head_dim;
-    const int left = s.keys - key0 < L::kKeys ? s.keys - key0 : L::kKeys;
-    const uint32_t bytes = next_there ? (left - 1) * row_bytes + a.head_dim * 2 : 0;
-    const auto k_page = page_rsrc(a.k + base, bytes), v_page = page_rsrc(a.v + base, bytes);
-#pragma unroll
-    for (int i = 0; i < L::kLoads; ++i) kst[i] = __builtin_amdgcn_raw_buffer_load_b128(k_page, from, i * L::kStep * row_bytes, 0);
-#pragma unroll
-    for (int i = 0; i < L::kLoads; ++i) vst[i] = __builtin_amdgcn_raw_buffer_load_b128(v_page, from, i * L::kStep * row_bytes, 0);
+  // A key tile's place in the pools and its bytes, up to the request's last row:
+  // zeros come from behind it, whatever the page holds there, and for tiles behind
+  // the last one or of pages outside the pool.  It is worked out in four steps of
+  // a few scalar instructions, which the gaps between two products hide.
+  PagePlaces pages;
+  struct Place {
+    uint64_t from;
+    uint32_t bytes;
   };
+  struct Search {
+    int key0, lane;
+    uint32_t mask, in_page;
+    Place at;
+  };
+  const uint32_t head_bytes = head * a.head_dim * 2, row_end = a.head_dim * 2;
+  auto block_of = [&](int t) { return (range.tile(t < t_end ? t : t_end - 1) << L::kShift) >> kBlockShift; };
+  auto ready = [&](int t) KVC_INLINE {  // the page of tile t is in the lanes
+    const int block = t_end > 0 ? block_of(t) : 0;
+    if (!pages.covers(block)) pages.refill(a, table, block);
+  };
+  auto seek = [&](Search& f, int t, int step) KVC_INLINE {
+    if (step == 0) {
+      f.key0 = range.tile(t < t_end ? t : (t_end > 0 ? t_end - 1 : 0)) << L::kShift;
+      f.mask = t < t_end ? 0xffffffffu : 0;
+      f.lane = (f.key0 >> kBlockShift) - pages.first;
+    } else if (step == 1) {
+      f.at.from = static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(pages.high, f.lane))) << 32 |
+                  static_cast<uint32_t>(__builtin_amdgcn_readlane(pages.low, f.lane));
+      f.mask &= __builtin_amdgcn_readlane(pages.there, f.lane);
+    } else if (step == 2) {
+      f.in_page = (f.key0 & (kBlockSize - 1)) * row_bytes + head_bytes;
+      f.at.from += f.in_page;
+    } else {
+      const int left = s.keys - f.key0 < L::kKeys ? s.keys - f.key0 : L::kKeys;
+      f.at.bytes = ((left - 1) * row_bytes + row_end) & f.mask;
+    }
+  };
+  auto place_of = [&](int t) KVC_INLINE {
+    ready(t);
+    Search f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) seek(f, t, i);
+    return f.at;
+  };
+  auto load = [&](const uint16_t* pool, const Place& p, u32x4 (&to)[L::kLoads]) KVC_INLINE {
+    const auto tile = page_rsrc(pool, p.from, p.bytes);
+#pragma unroll
+    for (int i = 0; i < L::kLoads; ++i) to[i] = __builtin_amdgcn_raw_buffer_load_b128(tile, from, i * L::kStep * row_bytes, 0);
+  };
+  auto store_k = [&](int buffer) KVC_INLINE {
+    char* const to = reinterpret_cast<char*>(k_tile[buffer]);
+#pragma unroll
+    for (int i = 0; i < L::kLoads; ++i)
+      *reinterpret_cast<u32x4*>(to + (k_to ^ L::k_turn(i * L::kStep)) + i * L::kStep * L::kBytes) = kst[i];
+  };
+  auto store_v = [&](int buffer) KVC_INLINE {
+    char* const to = reinterpret_cast<char*>(v_tile[buffer]);
+#pragma unroll
+    for (int i = 0; i < L::kLoads; ++i) *reinterpret_cast<u32x4*>(to + v_to + i * L::kStep * L::kBytes) = vst[i];
+  };
+  // Of two groups of waves the second is half a tile behind the first, so one's
+  // products run beside the other's softmax.  A group loads what the first one
+  // needs in the next tile, which is one tile more ahead for the second.
+  const int group = L::kGroups > 1 ? wave >> 2 : 0;
 
+  const f32x16 kZero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
   f32x16 acc[kBlocks];
   float m_run, l_run;
   // A weight of zero turns an infinity or NaN among V into NaN for rows that do
   // not see it.  That shows in the outputs: a workgroup that finds one there
   // goes over its keys again with care.  Returns whether the thread has one.
-  auto go_over = [&](auto care) {
+  auto go_over = [&](auto care) KVC_INLINE {
   constexpr bool careful = decltype(care)::value;
 #pragma unroll
-  for (int b = 0; b < kBlocks; ++b) acc[b] = f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+  for (int b = 0; b < kBlocks; ++b) acc[b] = kZero;
   m_run = kNegInf;
   l_run = 0.0f;
-  if (t_begin < t_end) load(t_begin);
-  for (int t = t_begin; t < t_end; ++t) {
-    char* const kt = reinterpret_cast<char*>(k_tile[t & 1]);
-    char* const vt = reinterpret_cast<char*>(v_tile[t & 1]);
-    // No key of a page outside the pool is seen: its tile lies behind every row.
-    const int key0 = next_there ? range.tile(t) << L::kShift : 1 << 30;
+  // Weights of the tile before, and where its keys begin; none yet.
+  vec_t pf[kKeyBlocks][2];
 #pragma unroll
-    for (int i = 0; i < L::kLoads; ++i) {
-      *reinterpret_cast<u32x4*>(kt + (k_to ^ L::k_turn(i * L::kStep)) + i * L::kStep * L::kBytes) = kst[i];
-      *reinterpret_cast<u32x4*>(vt + v_to + i * L::kStep * L::kBytes) = vst[i];
-    }
-    // One barrier a tile: a wave past it has done with the other buffer, too.
-    __syncthreads();
-    load(t + 1);
-    const bool whole = key0 + L::kKeys <= first.end && (key0 >= last.low || key0 + L::kKeys <= a.sinks);
-
-    f32x16 sc[kKeyBlocks];
+  for (int kb = 0; kb < kKeyBlocks; ++kb) pf[kb][0] = pf[kb][1] = __builtin_bit_cast(vec_t, u32x4{0, 0, 0, 0});
+  int key0 = 0;
+  f32x16 sc[kKeyBlocks];
+  float tops[4];
+  // The products of a tile: S^T = K Q^T (if `scores`) from buffer `now`, then
+  // O^T += V^T P^T of the tile before, from buffer `before`.  A left operand is
+  // read kAhead products before its use, and the order is the source's (left to
+  // itself the compiler reads one into the registers that the product before has
+  // just freed, and each waits for LDS).  beside(i) is done between products.
+  constexpr int kScores = kKeyBlocks * kSteps, kValues = kKeyBlocks * 2 * kBlocks;
+  constexpr int kAhead = L::kGroups > 1 ? 4 : 8;  // a second wave on the SIMD hides the rest
+  vec_t ring[kAhead];
+  auto k_operand = [&](int buffer, int i) KVC_INLINE {
+    const char* at = reinterpret_cast<const char*>(k_tile[buffer]) + (k_from ^ (i / kKeyBlocks << 5)) + (i % kKeyBlocks) * 32 * L::kBytes;
+    return __builtin_bit_cast(vec_t, *reinterpret_cast<const u32x4*>(at));
+  };
+  auto v_operand = [&](int buffer, int i) KVC_INLINE {
+    const char* at = reinterpret_cast<const char*>(v_tile[buffer]) + (v_from ^ (i % kBlocks << 6)) + (i / kBlocks) * 16 * L::kBytes;
+    return join_columns<vec_t>(read_column(at), read_column(at + 8 * L::kBytes));
+  };
+  auto products = [&](auto scores, int now, int before, auto beside) KVC_INLINE {
+    constexpr int kFirst = decltype(scores)::value ? 0 : kScores, kAll = kScores + kValues;
+    auto operand = [&](int i) { return i < kScores ? k_operand(now, i) : v_operand(before, i - kScores); };
+    each<kFirst, kAll>([&](auto step) KVC_INLINE {
+      constexpr int i = decltype(step)::value;
+      __builtin_amdgcn_sched_barrier(0);
+      vec_t left = ring[(i - kFirst) % kAhead];
+      if constexpr (i < kScores) {
+        const int kb = i % kKeyBlocks, st = i / kKeyBlocks;
+        sc[kb] = E::mfma32(left, qf[st], st ? sc[kb] : kZero);
+      } else {
+        const int b = (i - kScores) % kBlocks, kh = (i - kScores) / kBlocks, kb = kh >> 1, h = kh & 1;
+        if constexpr (careful) {
+          // Values that are not finite are added only to the rows that see them,
+          // token by token.
+          s16x8 raw = __builtin_bit_cast(s16x8, left), odd = {0, 0, 0, 0, 0, 0, 0, 0};
+          bool any = false;
 #pragma unroll
-    for (int kb = 0; kb < kKeyBlocks; ++kb) {
-      sc[kb] = f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+          for (int j = 0; j < 8; ++j)
+            if ((static_cast<uint16_t>(raw[j]) & E::kExponent) == E::kExponent) {
+              odd[j] = raw[j];
+              raw[j] = 0;
+              any = true;
+            }
+          left = __builtin_bit_cast(vec_t, raw);
+          if (__any(any)) {
+            for (int n = token_first; n <= token_last; ++n) {
+              const RowSight one = sight_of(a, s, place0 + n);
+              s16x8 seen = odd;
 #pragma unroll
-      for (int st = 0; st < kSteps; ++st) {
-        const vec_t kf = __builtin_bit_cast(
-            vec_t, *reinterpret_cast<const u32x4*>(kt + (k_from ^ (st << 5)) + kb * 32 * L::kBytes));
-        sc[kb] = E::mfma32(kf, qf[st], sc[kb]);
+              for (int j = 0; j < 8; ++j)
+                if (!sees(one, a.sinks, key0 + kb * 32 + h * 16 + 8 * (j >> 2) + 4 * half + (j & 3))) seen[j] = 0;
+              const f32x16 more = E::mfma32(__builtin_bit_cast(vec_t, seen), pf[kb][h], kZero);
+              if (token == n) acc[b] += more;
+            }
+          }
+        }
+        acc[b] = E::mfma32(left, pf[kb][h], acc[b]);
       }
+      if (i + kAhead < kAll) ring[(i - kFirst) % kAhead] = operand(i + kAhead);
+      beside(i);
+    });
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // The maximum of a lane's scores, in four chains (one would wait for itself).
+  auto top_of = [&](int e) KVC_INLINE { tops[e & 3] = fmaxf(tops[e & 3], sc[e >> 4][e & 15]); };
+  auto all_tops = [&]() KVC_INLINE { return max_across_halves(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]))); };
+  constexpr int kLane = kKeyBlocks * 16;  // scores of a lane
+
+  // The first tile of K, a tile of zeros as V before it, and what the second group
+  // stores ahead; the next ones wait in registers.
+  int now = 0, next = 1, before = 2;  // buffers of tiles t, t + 1 and t - 1
+  Place old = place_of(t_begin);
+  uint32_t there = old.bytes != 0;  // whether the last tiles that were asked for are in the pool, the latest lowest
+  load(a.k, old, kst);
+  store_k(now);
+#pragma unroll
+  for (int i = 0; i < L::kLoads; ++i) vst[i] = u32x4{0, 0, 0, 0};
+  store_v(before);
+  Place ahead = place_of(t_begin + 1);
+  load(a.k, ahead, kst);
+  load(a.v, old, vst);
+  there = there << 1 | (ahead.bytes != 0);
+  old = ahead;
+  if (group) {
+    store_k(next);
+    store_v(now);
+    ahead = place_of(t_begin + 2);
+    load(a.k, ahead, kst);
+    load(a.v, old, vst);
+    there = there << 1 | (ahead.bytes != 0);
+    old = ahead;
+  }
+  ready(t_begin + 2 + group);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) ring[i] = k_operand(now, i);
+  if (group) __syncthreads();
+  for (int t = t_begin; t < t_end; ++t) {
+    // Products, beside them the tiles that wait in registers go to LDS, the ones
+    // behind those are asked for, and the scores' maximum is taken.
+    Search search;
+    float top;
+    tops[0] = tops[1] = tops[2] = tops[3] = kNegInf;
+    __builtin_amdgcn_s_setprio(1);
+    products(std::true_type{}, now, before, [&](int i) KVC_INLINE {
+      if (i == 1) store_k(group ? before : next);
+      if (i == 2) store_v(group ? next : now);
+      if (i >= 3 && i < 7) seek(search, t + 2 + group, i - 3);
+      if (i == 7) load(a.v, old, vst);
+      if (i == 8) load(a.k, search.at, kst);
+      constexpr int kFrom = kScores + 2, kTo = kScores + kValues;  // the scores are there
+#pragma unroll
+      for (int e = 0; e < kLane; ++e)
+        if (i == kFrom + e / 2 * 2 * (kTo - kFrom) / kLane) top_of(e);
+      if (i == kTo - 1) top = all_tops();
+    });
+    __builtin_amdgcn_s_setprio(0);
+    there = there << 1 | (search.at.bytes != 0);
+    old = search.at;
+    // No key of a page outside the pool is seen: its tile lies behind every row.
+    key0 = there >> (2 + group) & 1 ? range.tile(t) << L::kShift : 1 << 30;
+    __syncthreads();
+    __builtin_amdgcn_sched_barrier(0);
+    // Softmax.
+    if (!(key0 + L::kKeys <= first.end && (key0 >= last.low || key0 + L::kKeys <= a.sinks))) {
+      tops[0] = tops[1] = tops[2] = tops[3] = kNegInf;
+#pragma unroll
+      for (int e = 0; e < kLane; ++e) {
+        const int i = e & 15;
+        sc[e >> 4][i] = sees(sight, a.sinks, key0 + (e >> 4) * 32 + 8 * (i >> 2) + 4 * half + (i & 3)) ? sc[e >> 4][i] : kNegInf;
+        top_of(e);
+      }
+      top = all_tops();
     }
-    if (!whole) {
-#pragma unroll
-      for (int kb = 0; kb < kKeyBlocks; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          sc[kb][i] = sees(sight, a.sinks, key0 + kb * 32 + 8 * (i >> 2) + 4 * half + (i & 3)) ? sc[kb][i] : kNegInf;
-    }
-    float top = kNegInf;
-#pragma unroll
-    for (int kb = 0; kb < kKeyBlocks; ++kb)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[kb][i]);
-    top = max_across_halves(top) * a.scale_log2;
+    top *= a.scale_log2;
     // The maximum moves only when it grows by more than 2^8: weights then reach
     // 2^8 at most, and most tiles leave the outputs unscaled.
     const float m_new = top > m_run + 8.0f ? top : m_run;
@@ -270,8 +436,7 @@ __global__ __launch_bounds__(kManyThreads, many_residents(DP)) void attend_many_
       m_run = m_new;
     }
     const float m_use = m_run == kNegInf ? 0.0f : m_run;
-    vec_t pf[kKeyBlocks][2];
-    float sum = 0.0f;
+    float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int kb = 0; kb < kKeyBlocks; ++kb)
 #pragma unroll
@@ -281,52 +446,31 @@ __global__ __launch_bounds__(kManyThreads, many_residents(DP)) void attend_many_
         for (int j = 0; j < 8; j += 2) {
           const float p0 = exp2_fast(fmaf(sc[kb][8 * h + j], a.scale_log2, -m_use));
           const float p1 = exp2_fast(fmaf(sc[kb][8 * h + j + 1], a.scale_log2, -m_use));
-          sum += p0 + p1;
+          sums[j >> 1] += p0 + p1;
           w[j >> 1] = E::pack(p0, p1);
         }
         pf[kb][h] = __builtin_bit_cast(vec_t, w);
       }
-    l_run += sum;
-
+    l_run += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    ready(t + 3 + group);
+    // The next products' first operands: they have been there for a phase.
+    const int free = before;
+    before = now;
+    now = next;
+    next = free;
 #pragma unroll
-    for (int kb = 0; kb < kKeyBlocks; ++kb)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int b = 0; b < kBlocks; ++b) {
-          const char* at = vt + (v_from ^ (b << 6)) + (kb * 32 + h * 16) * L::kBytes;
-          const s16x4 v0 = read_column(at);
-          const s16x4 v1 = read_column(at + 8 * L::kBytes);
-          vec_t vf = join_columns<vec_t>(v0, v1);
-          if constexpr (careful) {
-            // Values that are not finite are added only to the rows that see
-            // them, token by token.
-            s16x8 raw = __builtin_bit_cast(s16x8, vf), odd = {0, 0, 0, 0, 0, 0, 0, 0};
-            bool any = false;
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if ((static_cast<uint16_t>(raw[j]) & E::kExponent) == E::kExponent) {
-                odd[j] = raw[j];
-                raw[j] = 0;
-                any = true;
-              }
-            vf = __builtin_bit_cast(vec_t, raw);
-            if (__any(any)) {
-              for (int i = token_first; i <= token_last; ++i) {
-                const RowSight one = sight_of(a, s, place0 + i);
-                s16x8 seen = odd;
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                  if (!sees(one, a.sinks, key0 + kb * 32 + h * 16 + 8 * (j >> 2) + 4 * half + (j & 3))) seen[j] = 0;
-                const f32x16 more =
-                    E::mfma32(__builtin_bit_cast(vec_t, seen), pf[kb][h], f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0});
-                if (token == i) acc[b] += more;
-              }
-            }
-          }
-          acc[b] = E::mfma32(vf, pf[kb][h], acc[b]);
-        }
+    for (int i = 0; i < kAhead; ++i) ring[i] = k_operand(now, i);
+    __builtin_amdgcn_sched_barrier(0);
+    // Nothing was stored since the last barrier: no wait for LDS before this one.
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
   }
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) ring[i] = v_operand(before, i);
+  products(std::false_type{}, now, before, [](int) {});
+  if (L::kGroups > 1 && !group) __syncthreads();
   bool wild = false;
 #pragma unroll
   for (int b = 0; b < kBlocks; ++b)
@@ -351,7 +495,7 @@ __global__ __launch_bounds__(kManyThreads, many_residents(DP)) void attend_many_
               u32x2{E::pack(acc[b][4 * i] * inv, acc[b][4 * i + 1] * inv), E::pack(acc[b][4 * i + 2] * inv, acc[b][4 * i + 3] * inv)};
       }
   } else {
-    float* const piece = a.partial + ((static_cast<int64_t>(item) * a.kv_heads + head) * splits + split) * piece_floats(kManyRows, DP);
+    float* const piece = a.partial + ((static_cast<int64_t>(item) * a.kv_heads + head) * splits + split) * piece_floats(kRows, DP);
     const int local = m - row0;
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b)
@@ -359,30 +503,31 @@ __global__ __launch_bounds__(kManyThreads, many_residents(DP)) void attend_many_
       for (int i = 0; i < 4; ++i)
         *gptr(reinterpret_cast<f32x4*>(piece + local * DP + b * 32 + i * 8 + half * 4)) =
             f32x4{acc[b][4 * i], acc[b][4 * i + 1], acc[b][4 * i + 2], acc[b][4 * i + 3]};
-    if (half == 0) *gptr(reinterpret_cast<f32x2*>(piece + kManyRows * DP + 2 * local)) = f32x2{m_run, l_all};
+    if (half == 0) *gptr(reinterpret_cast<f32x2*>(piece + kRows * DP + 2 * local)) = f32x2{m_run, l_all};
   }
 }
 
 // Joins the splits of a (row tile, KV head), 16 rows a workgroup, four at a time.
 template <bool F16, int DP>
-__global__ __launch_bounds__(kManyThreads) void attend_many_join_kernel(AttendArgs a, ManyGrid grid) {
+__global__ __launch_bounds__(kJoinThreads) void attend_many_join_kernel(AttendArgs a, ManyGrid grid) {
   typedef AttendElem<F16> E;
+  constexpr int kRows = many_rows(DP);
   const int head = blockIdx.x % a.kv_heads, item = blockIdx.x / a.kv_heads;
-  const TileCount counted(a);
+  const TileCount<kRows> counted(a);
   const ManyShares shares(a, grid, counted.total());
   const int tile = shares.total - 1 - shares.whole - item;
   if (tile < 0) return;
   int request, local_tile;
   counted.find(a, tile, &request, &local_tile);
   const Request s = uniform_request_of(a, request);
-  const int row0 = local_tile * kManyRows, left = s.fresh * a.qpk - row0;
-  const int64_t size = piece_floats(kManyRows, DP);
+  const int row0 = local_tile * kRows, left = s.fresh * a.qpk - row0;
+  const int64_t size = piece_floats(kRows, DP);
   const float* const pieces = a.partial + (static_cast<int64_t>(item) * a.kv_heads + head) * shares.splits * size;
   const int begin = blockIdx.y * 16, end = left < begin + 16 ? left : begin + 16;
   for (int row = begin; row < end; row += 4) {
     if (row > begin) __syncthreads();
     join_pieces<DP>(
-        shares.splits, row, end, a.head_dim, kManyRows * DP, [&](int i) { return pieces + i * size; },
+        shares.splits, row, end, a.head_dim, kRows * DP, [&](int i) { return pieces + i * size; },
         [&](int local, int d, f32x4 x) {
           const int m = row0 + local, token = m / a.qpk, g = m - token * a.qpk;
           uint16_t* to = a.out + (s.token0 + token) * a.out_token_stride + (head * a.qpk + g) * a.out_head_stride;
@@ -393,11 +538,12 @@ __global__ __launch_bounds__(kManyThreads) void attend_many_join_kernel(AttendAr
 
 template <bool F16, int DP>
 int launch(hipStream_t stream, const AttendArgs& a, const ManyGrid& grid) {
-  attend_many_kernel<F16, DP><<<static_cast<unsigned>(grid.grid), kManyThreads, 0, stream>>>(a, grid);
+  constexpr int kRows = many_rows(DP);
+  attend_many_kernel<F16, DP><<<static_cast<unsigned>(grid.grid), ManyLayout<DP>::kThreads, 0, stream>>>(a, grid);
   if (int rc = launch_status("kvc_attend_paged")) return rc;
   // Split items number half a round at most: each has two splits or more.
   if (grid.most_splits > 1)
-    attend_many_join_kernel<F16, DP><<<dim3(grid.round / 2, kManyRows / 16), kManyThreads, 0, stream>>>(a, grid);
+    attend_many_join_kernel<F16, DP><<<dim3(grid.round / 2, kRows / 16), kJoinThreads, 0, stream>>>(a, grid);
   return launch_status("kvc_attend_paged");
 }
 
