@@ -24,14 +24,19 @@ AttendPlan make_plan(int kv_heads, int qpk, int head_dim, int n_seq, int64_t num
   const int64_t most_rows = static_cast<int64_t>(max_query_len) * qpk;
   const int64_t pages = ceil_div(max_seq_len > 0 ? max_seq_len : 1, kBlockSize);
   size_t few = 0, many = 0;
-  // A lone request of many rows leaves the few-rows kernel nothing; whatever its
-  // real length, the many-rows kernel takes it.
-  const bool lone = n_seq == 1 && most_rows > kFewRows * kFewTilesMost;
-  if (qpk <= kFewRows * kFewTilesMost && !lone) {
+  // A small batch that needs the many-rows kernel leaves it the few rows too: its
+  // padding costs less than a launch of each kind.  Requests of one to four tokens
+  // (8 heads each) beside a chunk of 256, head_dim 64 / 128 / 256:
+  //   7 of 4096 keys, 2 KV heads   40 / 48 / 67 us, apart 60 / 75 / 100
+  //   31 of 2048, 8 KV heads       70 / 97 / 158,   apart 89 / 114 / 176
+  //   63 of 4096, 8 KV heads       195 / 298 / 480, apart 185 / 263 / 482
+  const bool together = most_rows > kFewRows * kFewTilesMost &&
+                        static_cast<int64_t>(n_seq) * kv_heads * max_seq_len <= (1 << 19);
+  if (qpk <= kFewRows * kFewTilesMost && !together) {
     p.row_tiles = most_rows <= kFewRows ? 1 : kFewTilesMost;
     p.sequences = n_seq < kFewSequences ? n_seq : kFewSequences;
     const int64_t bound = static_cast<int64_t>(p.sequences) * kv_heads * pages;
-    const int64_t resident = kCompute * few_residents(dim, p.row_tiles);
+    const int64_t resident = kCompute * few_residents(dim);
     p.workgroups = static_cast<int>(bound < resident ? bound : resident);
     few = static_cast<size_t>(p.workgroups) * (16 + 8 * piece_floats(kFewRows * p.row_tiles, dim));
   }

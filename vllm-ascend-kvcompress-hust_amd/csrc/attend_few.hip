@@ -49,7 +49,7 @@ struct FewLayout {
 // the outputs, the queries, and a slice's K and V ahead of their use; each wave
 // then has 64 x DP bytes in flight.
 template <bool F16, int DP, int NQ>
-__global__ __launch_bounds__(kFewThreads, few_residents(DP, NQ)) void attend_few_kernel(AttendArgs a) {
+__global__ __launch_bounds__(kFewThreads, few_residents(DP)) void attend_few_kernel(AttendArgs a) {
   typedef AttendElem<F16> E;
   typedef typename E::vec vec_t;
   constexpr int kSteps = DP / 32;   // 32-dim steps of K Q^T
@@ -57,6 +57,10 @@ __global__ __launch_bounds__(kFewThreads, few_residents(DP, NQ)) void attend_few
   constexpr int kRows = 16 * NQ;
   typedef FewLayout<DP> Layout;
   __shared__ __attribute__((aligned(16))) uint16_t v_stage[kFewWaves][kSliceKeys * Layout::kRow];
+  // Two row tiles' queries are read from LDS where they are used, in operand
+  // order: in registers they left too few for the loads ahead (XXX).
+  constexpr bool kQueriesHeld = NQ == 1;
+  __shared__ u32x4 q_stage[kQueriesHeld ? 1 : NQ * kSteps * 64];
   __shared__ int before[kFewSequences + 1];
   __shared__ float wave_m[kFewWaves][kRows], wave_l[kFewWaves][kRows];
   __shared__ int wave_sum[kFewWaves];
@@ -134,7 +138,7 @@ __global__ __launch_bounds__(kFewThreads, few_residents(DP, NQ)) void attend_few
     const int rows = s.fresh * a.qpk;
     const int place0 = s.len - s.fresh;
 
-    vec_t qf[NQ][kSteps];
+    vec_t qf[kQueriesHeld ? kSteps : 1];
     RowSight sight[NQ];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
@@ -150,10 +154,21 @@ __global__ __launch_bounds__(kFewThreads, few_residents(DP, NQ)) void attend_few
       for (int st = 0; st < kSteps; ++st) {
         const int d = st * 32 + group * 8;
         u32x4 w = {0, 0, 0, 0};
+        if (!kQueriesHeld && (n * kSteps + st) % kFewWaves != wave) continue;
         if (inside && d < a.head_dim) w = *gptr(reinterpret_cast<const u32x4*>(row + d));
-        qf[n][st] = __builtin_bit_cast(vec_t, w);
+        if constexpr (kQueriesHeld)
+          qf[st] = __builtin_bit_cast(vec_t, w);
+        else
+          q_stage[(n * kSteps + st) * 64 + lane] = w;
       }
     }
+    if constexpr (!kQueriesHeld) __syncthreads();
+    auto query = [&](int n, int st) {
+      if constexpr (kQueriesHeld)
+        return qf[st];
+      else
+        return __builtin_bit_cast(vec_t, q_stage[(n * kSteps + st) * 64 + lane]);
+    };
     __builtin_amdgcn_s_waitcnt(0x0f70);  // the queries are there: the loop's waits count its own loads alone
     // Keys that some row sees, and those that every row sees.
     const int last_end = place0 + s.fresh < s.keys ? place0 + s.fresh : s.keys;
@@ -225,6 +240,9 @@ __global__ __launch_bounds__(kFewThreads, few_residents(DP, NQ)) void attend_few
     }
     while (now.tile < piece_last) {
       const int key0 = now.key0;
+      // Worked out anew: places held through the loop are registers that loads ahead need.
+      int to = v_to, column = v_from;
+      asm volatile("" : "+v"(to), "+v"(column));
       const bool whole = key0 + kSliceKeys <= first_end && (key0 >= last_low || key0 + kSliceKeys <= a.sinks);
       const Slice next = find(now.tile + 1);
       if (a.head_dim != DP) {
@@ -242,9 +260,9 @@ __global__ __launch_bounds__(kFewThreads, few_residents(DP, NQ)) void attend_few
         for (int b = 0; b < 2; ++b) {
           sc[n][b] = f32x4{0, 0, 0, 0};
 #pragma unroll
-          for (int st = 0; st < kSteps; ++st) sc[n][b] = E::mfma(__builtin_bit_cast(vec_t, kw[b][st]), qf[n][st], sc[n][b]);
+          for (int st = 0; st < kSteps; ++st) sc[n][b] = E::mfma(__builtin_bit_cast(vec_t, kw[b][st]), query(n, st), sc[n][b]);
         }
-      if (next.tile < piece_last) load_k(next);
+      if (!careful && next.tile < piece_last) load_k(next);
 
       vec_t hi[NQ], lo[NQ];
 #pragma unroll
@@ -284,13 +302,13 @@ __global__ __launch_bounds__(kFewThreads, few_residents(DP, NQ)) void attend_few
       }
 
 #pragma unroll
-      for (int i = 0; i < Layout::kLoads; ++i) *reinterpret_cast<u32x4*>(stage + Layout::chunk_at(v_to, i)) = vw[i];
-      if (next.tile < piece_last) load_v(next);
+      for (int i = 0; i < Layout::kLoads; ++i) *reinterpret_cast<u32x4*>(stage + Layout::chunk_at(to, i)) = vw[i];
+      if (!careful && next.tile < piece_last) load_v(next);
       // The wave reads what it wrote itself: its LDS operations keep their order.
       __builtin_amdgcn_wave_barrier();
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b) {
-        const char* from = stage + (v_from ^ ((b & 7) << 5)) + (b >> 3) * 256;
+        const char* from = stage + (column ^ ((b & 7) << 5)) + (b >> 3) * 256;
         const s16x4 v0 = read_column(from);
         const s16x4 v1 = read_column(from + 16 * Layout::kRow * 2);
         vec_t vf = join_columns<vec_t>(v0, v1);
@@ -329,6 +347,10 @@ __global__ __launch_bounds__(kFewThreads, few_residents(DP, NQ)) void attend_few
         }
       }
       __builtin_amdgcn_wave_barrier();
+      if (careful && next.tile < piece_last) {  // not ahead: registers that the fast pass has no use for
+        load_k(next);
+        load_v(next);
+      }
       now = next;
     }
     bool wild = false;
@@ -446,7 +468,7 @@ __global__ __launch_bounds__(kFewThreads) void attend_few_join_kernel(AttendArgs
   const int64_t size = piece_floats(kRows, DP);
   const float* const first = a.partial + (2 * static_cast<int64_t>(wg) + kind) * size;
   const float* const rest = a.partial + 2 * static_cast<int64_t>(wg) * size;  // piece i > 0 at 2*i*size
-  join_pieces<DP>(
+  join_pieces<DP, 4>(
       count, row0, rows, a.head_dim, kRows * DP, [&](int i) { return i ? rest + 2 * i * size : first; },
       [&](int m, int d, f32x4 x) {
         const int token = m / a.qpk, g = m - token * a.qpk;

@@ -189,56 +189,64 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 
 constexpr float kNegInf = -__builtin_inff();
 
-// Joins `count` pieces of four rows (first, first + 1, .. below `rows`) of which
+// Joins `count` pieces of ROWS rows (first, first + 1, .. below `rows`) of which
 // piece i is at piece(i): `floats` unnormalised outputs of DP dims a row, then
-// (maximum, sum) pairs.  A workgroup of 256: a wave a row finds the common
-// maximum and sum, then every thread adds four dims of some of the pieces, and
-// the shares meet in LDS.  store(row, dim, f32x4) takes the results.
-template <int DP, typename Piece, typename Store>
+// (maximum, sum) pairs.  A workgroup of 256: 256 / ROWS lanes a row find the common
+// maximum and sum, then every thread adds four dims at a time of all or of every
+// other piece, and such shares meet in LDS.  store(row, dim, f32x4) takes the
+// results.
+template <int DP, int ROWS, typename Piece, typename Store>
 __device__ __forceinline__ void join_pieces(int count, int first, int rows, int head_dim, int floats, Piece piece, Store store) {
-  constexpr int kUnits = DP;  // four rows of DP / 4 units
-  constexpr int kShares = kUnits <= 128 ? 2 : 1;
-  __shared__ float top_of[4], inv_of[4];
+  constexpr int kUnits = ROWS * DP / 4, kLanes = 256 / ROWS;
+  constexpr int kShares = kUnits <= 128 ? 2 : 1, kEach = (kUnits + 255) / 256;
+  __shared__ float top_of[ROWS], inv_of[ROWS];
   __shared__ f32x4 shared_sum[kShares > 1 ? 256 : 1];
-  const int lane = threadIdx.x & 63, own = first + (threadIdx.x >> 6);
+  const int tid = threadIdx.x, lane = tid % kLanes, own = first + tid / kLanes;
   if (own < rows) {
     float top = kNegInf;
-    for (int i = lane; i < count; i += 64) top = fmaxf(top, piece(i)[floats + 2 * own]);
+    for (int i = lane; i < count; i += kLanes) top = fmaxf(top, piece(i)[floats + 2 * own]);
 #pragma unroll
-    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    for (int d = kLanes / 2; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
     const float use = top == kNegInf ? 0.0f : top;
     float sum = 0.0f;
-    for (int i = lane; i < count; i += 64) {
+    for (int i = lane; i < count; i += kLanes) {
       const f32x2 ml = *reinterpret_cast<const f32x2*>(piece(i) + floats + 2 * own);
       sum += ml[1] * exp2_fast(ml[0] - use);
     }
 #pragma unroll
-    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+    for (int d = kLanes / 2; d; d >>= 1) sum += __shfl_xor(sum, d);
     if (lane == 0) {
       top_of[own - first] = use;
       inv_of[own - first] = sum == 0.0f ? 0.0f : 1.0f / sum;
     }
   }
   __syncthreads();
-  const int share = threadIdx.x / kUnits, unit = threadIdx.x - share * kUnits;
-  const int local = unit / (DP / 4), d = (unit - local * (DP / 4)) * 4, row = first + local;
-  const bool working = share < kShares && row < rows && d < head_dim;
-  f32x4 sum = {0, 0, 0, 0};
-  if (working) {
-    const float use = top_of[local];
+  f32x4 sums[kEach];
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int share = kShares > 1 ? tid / kUnits : 0, unit = tid + e * 256 - share * kUnits;
+    const int local = unit / (DP / 4), d = (unit - local * (DP / 4)) * 4, row = first + local;
+    sums[e] = f32x4{0, 0, 0, 0};
+    if (share < kShares && unit < kUnits && row < rows && d < head_dim) {
+      const float use = top_of[local];
 #pragma unroll 8
-    for (int i = share; i < count; i += kShares) {
-      const float* p = piece(i);
-      sum += *reinterpret_cast<const f32x4*>(p + row * DP + d) * exp2_fast(p[floats + 2 * row] - use);
+      for (int i = share; i < count; i += kShares) {
+        const float* p = piece(i);
+        sums[e] += *reinterpret_cast<const f32x4*>(p + row * DP + d) * exp2_fast(p[floats + 2 * row] - use);
+      }
+      sums[e] *= inv_of[local];
     }
-    sum *= inv_of[local];
   }
   if constexpr (kShares > 1) {
-    if (share == 1) shared_sum[unit] = sum;
+    if (tid >= kUnits && tid < 2 * kUnits) shared_sum[tid - kUnits] = sums[0];
     __syncthreads();
-    if (share == 0) sum += shared_sum[unit];
+    if (tid < kUnits) sums[0] += shared_sum[tid];
   }
-  if (working && share == 0) store(row, d, sum);
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int unit = tid + e * 256, local = unit / (DP / 4), d = (unit - local * (DP / 4)) * 4, row = first + local;
+    if (unit < kUnits && row < rows && d < head_dim) store(row, d, sums[e]);
+  }
 }
 
 // The many-rows launch: `round` workgroups fit the device at once, `grid` are
@@ -260,7 +268,7 @@ constexpr int kFewSequences = 1024;  // requests of one launch (their prefix sum
 constexpr int many_rows(int dim) { return dim <= 128 ? 256 : 128; }
 
 // Few-rows workgroups that a compute unit holds.
-constexpr int few_residents(int dim, int row_tiles) { return dim <= 64 ? 4 - row_tiles : (dim <= 128 ? 2 : 1); }
+constexpr int few_residents(int dim) { return dim <= 64 ? 3 : (dim <= 128 ? 2 : 1); }
 
 // Floats of a piece of `rows` rows: unnormalised outputs, then (max, sum) pairs.
 __host__ __device__ inline int64_t piece_floats(int rows, int dim) { return static_cast<int64_t>(rows) * (dim + 2); }

@@ -34,7 +34,7 @@ __device__ __forceinline__ void each(F f) {
   each_of<FROM>(std::make_integer_sequence<int, TO - FROM>{}, f);
 }
 
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 256, kJoinRows = 16;
 
 // K's and V's place in LDS: rows of 64, 128 or 256 elements whose 16-byte chunks
 // are moved, by an exclusive or with a number of the row, so that the 16 rows of
@@ -507,7 +507,7 @@ __global__ __launch_bounds__(ManyLayout<DP>::kThreads, ManyLayout<DP>::kGroups) 
   }
 }
 
-// Joins the splits of a (row tile, KV head), 16 rows a workgroup, four at a time.
+// Joins the splits of a (row tile, KV head), kJoinRows rows a workgroup.
 template <bool F16, int DP>
 __global__ __launch_bounds__(kJoinThreads) void attend_many_join_kernel(AttendArgs a, ManyGrid grid) {
   typedef AttendElem<F16> E;
@@ -523,17 +523,15 @@ __global__ __launch_bounds__(kJoinThreads) void attend_many_join_kernel(AttendAr
   const int row0 = local_tile * kRows, left = s.fresh * a.qpk - row0;
   const int64_t size = piece_floats(kRows, DP);
   const float* const pieces = a.partial + (static_cast<int64_t>(item) * a.kv_heads + head) * shares.splits * size;
-  const int begin = blockIdx.y * 16, end = left < begin + 16 ? left : begin + 16;
-  for (int row = begin; row < end; row += 4) {
-    if (row > begin) __syncthreads();
-    join_pieces<DP>(
-        shares.splits, row, end, a.head_dim, kRows * DP, [&](int i) { return pieces + i * size; },
-        [&](int local, int d, f32x4 x) {
-          const int m = row0 + local, token = m / a.qpk, g = m - token * a.qpk;
-          uint16_t* to = a.out + (s.token0 + token) * a.out_token_stride + (head * a.qpk + g) * a.out_head_stride;
-          *gptr(reinterpret_cast<u32x2*>(to + d)) = u32x2{E::pack(x[0], x[1]), E::pack(x[2], x[3])};
-        });
-  }
+  const int begin = blockIdx.y * kJoinRows;
+  join_pieces<DP, kJoinRows>(
+      shares.splits, begin, left < begin + kJoinRows ? left : begin + kJoinRows, a.head_dim, kRows * DP,
+      [&](int i) { return pieces + i * size; },
+      [&](int local, int d, f32x4 x) {
+        const int m = row0 + local, token = m / a.qpk, g = m - token * a.qpk;
+        uint16_t* to = a.out + (s.token0 + token) * a.out_token_stride + (head * a.qpk + g) * a.out_head_stride;
+        *gptr(reinterpret_cast<u32x2*>(to + d)) = u32x2{E::pack(x[0], x[1]), E::pack(x[2], x[3])};
+      });
 }
 
 template <bool F16, int DP>
@@ -543,7 +541,7 @@ int launch(hipStream_t stream, const AttendArgs& a, const ManyGrid& grid) {
   if (int rc = launch_status("kvc_attend_paged")) return rc;
   // Split items number half a round at most: each has two splits or more.
   if (grid.most_splits > 1)
-    attend_many_join_kernel<F16, DP><<<dim3(grid.round / 2, kRows / 16), kJoinThreads, 0, stream>>>(a, grid);
+    attend_many_join_kernel<F16, DP><<<dim3(grid.round / 2, kRows / kJoinRows), kJoinThreads, 0, stream>>>(a, grid);
   return launch_status("kvc_attend_paged");
 }
 
