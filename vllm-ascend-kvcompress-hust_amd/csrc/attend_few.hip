@@ -135,6 +135,7 @@ __global__ __launch_bounds__(kFewThreads, few_residents(DP)) void attend_few_ker
     const int piece_first = at - whole_begin;
     const int piece_end = whole_begin + tiles < range_end ? whole_begin + tiles : range_end;
     const int piece_last = piece_end - whole_begin;
+    const int32_t* const table = a.table + r * a.table_stride;
     const int rows = s.fresh * a.qpk;
     const int place0 = s.len - s.fresh;
 
@@ -169,7 +170,11 @@ __global__ __launch_bounds__(kFewThreads, few_residents(DP)) void attend_few_ker
       else
         return __builtin_bit_cast(vec_t, q_stage[(n * kSteps + st) * 64 + lane]);
     };
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // the queries are there: the loop's waits count its own loads alone
+    // The first pages' numbers beside the queries, both there before the loop: its
+    // waits count its own loads alone.
+    PageIds ids;
+    ids.fill(table, a.max_blocks, pages.count() ? pages.tile(piece_first) : 0);
+    __builtin_amdgcn_s_waitcnt(0x0f70);
     // Keys that some row sees, and those that every row sees.
     const int last_end = place0 + s.fresh < s.keys ? place0 + s.fresh : s.keys;
     const int first_end = place0 + 1 < s.keys ? place0 + 1 : s.keys;
@@ -182,8 +187,6 @@ __global__ __launch_bounds__(kFewThreads, few_residents(DP)) void attend_few_ker
       int tile, key0;
       uint64_t base;  // bytes
     };
-    const int32_t* const table = a.table + r * a.table_stride;
-    PageIds ids;
     auto find = [&](int t) {
       Slice f = {t, 0, 0};
       if (pages.count() == 0) f.tile = piece_last;
@@ -440,10 +443,10 @@ __global__ __launch_bounds__(kFewThreads, few_residents(DP)) void attend_few_ker
       }
       if (!complete && piece_first == 0 && lane == 0) {
         // The (request, head) goes on in the next workgroups: `count` pieces in all.
-        a.header[4 * wg] = r;
-        a.header[4 * wg + 1] = head;
+        a.header[4 * wg] = s.token0;
+        a.header[4 * wg + 1] = rows;
         a.header[4 * wg + 2] = (whole_begin + tiles - 1) / per - wg + 1;
-        a.header[4 * wg + 3] = kind;
+        a.header[4 * wg + 3] = head << 1 | kind;
       }
     }
     at = piece_end;
@@ -461,9 +464,8 @@ __global__ __launch_bounds__(kFewThreads) void attend_few_join_kernel(AttendArgs
   const int wg = blockIdx.x, row0 = blockIdx.y * 4;
   const int count = scalar_at(a.header, 4 * wg + 2);
   if (count < 2) return;
-  const int r = scalar_at(a.header, 4 * wg), head = scalar_at(a.header, 4 * wg + 1), kind = scalar_at(a.header, 4 * wg + 3);
-  const Request s = uniform_request_of(a, r);
-  const int rows = s.fresh * a.qpk;
+  const int token0 = scalar_at(a.header, 4 * wg), rows = scalar_at(a.header, 4 * wg + 1);
+  const int head = scalar_at(a.header, 4 * wg + 3) >> 1, kind = scalar_at(a.header, 4 * wg + 3) & 1;
   if (row0 >= rows) return;
   const int64_t size = piece_floats(kRows, DP);
   const float* const first = a.partial + (2 * static_cast<int64_t>(wg) + kind) * size;
@@ -472,7 +474,7 @@ __global__ __launch_bounds__(kFewThreads) void attend_few_join_kernel(AttendArgs
       count, row0, rows, a.head_dim, kRows * DP, [&](int i) { return i ? rest + 2 * i * size : first; },
       [&](int m, int d, f32x4 x) {
         const int token = m / a.qpk, g = m - token * a.qpk;
-        uint16_t* to = a.out + (s.token0 + token) * a.out_token_stride + (head * a.qpk + g) * a.out_head_stride;
+        uint16_t* to = a.out + (token0 + token) * a.out_token_stride + (head * a.qpk + g) * a.out_head_stride;
         *gptr(reinterpret_cast<u32x2*>(to + d)) = u32x2{E::pack(x[0], x[1]), E::pack(x[2], x[3])};
       });
 }

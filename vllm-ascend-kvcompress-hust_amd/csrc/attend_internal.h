@@ -142,14 +142,15 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 // A request's pages, 64 at a time in the wave's lanes: a page's number then costs
 // no wait.  -1 where the table ends.
 struct PageIds {
-  int first = -(1 << 30), ids = -1;
+  int first, ids;
+  __device__ __forceinline__ void fill(const int32_t* table, int max_blocks, int block) {
+    first = block;
+    const int mine = block + static_cast<int>(threadIdx.x & 63);
+    ids = mine < max_blocks ? *gptr(table + mine) : -1;
+    asm volatile("" : "+v"(ids));  // waited for here, not wherever it is used
+  }
   __device__ __forceinline__ int at(const int32_t* table, int max_blocks, int block) {
-    if (block - first >= 64 || block < first) {
-      first = block;
-      const int mine = block + static_cast<int>(threadIdx.x & 63);
-      ids = mine < max_blocks ? *gptr(table + mine) : -1;
-      asm volatile("" : "+v"(ids));  // waited for here, not wherever it is used
-    }
+    if (block - first >= 64 || block < first) fill(table, max_blocks, block);
     return __builtin_amdgcn_readlane(ids, block - first);
   }
 };

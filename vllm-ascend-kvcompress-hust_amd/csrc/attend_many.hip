@@ -51,20 +51,17 @@ struct ManyLayout {
   static constexpr int kSlots = kRow / 8;
   static constexpr int kGroups = many_rows(DP) / 128;  // of four waves, 32 rows each
   static constexpr int kThreads = 256 * kGroups;
+  static constexpr int kBuffers = kGroups > 1 ? 3 : 2;  // of K and of V in LDS
   static constexpr int kStep = kThreads / kSlots;
   static constexpr int kLoads = kKeys / kStep;
   __device__ __forceinline__ static constexpr int k_turn(int row) { return (kRow == 64 ? (row >> 1) & 7 : row & 15) << 4; }
   __device__ __forceinline__ static constexpr int v_turn(int row) { return (kRow == 64 ? (row >> 1) & 1 : row & 3) << 6; }
 };
 
-// Row tiles of request r that are this kernel's.
+// Row tiles of a request that are this kernel's.
 template <int ROWS>
-__device__ __forceinline__ int tiles_of(const AttendArgs& a, int r) {
-  const int64_t total = a.num_tokens;
-  int64_t t0 = a.start[r], t1 = a.start[r + 1];
-  t0 = t0 < 0 ? 0 : (t0 > total ? total : t0);
-  t1 = t1 < t0 ? t0 : (t1 > total ? total : t1);
-  const int64_t rows = (t1 - t0) * a.qpk;
+__device__ __forceinline__ int tiles_of(const AttendArgs& a, const Request& s) {
+  const int64_t rows = static_cast<int64_t>(s.fresh) * a.qpk;
   return rows > a.few_rows ? static_cast<int>((rows + ROWS - 1) / ROWS) : 0;
 }
 
@@ -82,30 +79,40 @@ __device__ __forceinline__ int sum_up_to_lane(int x) {
 template <int ROWS>
 struct TileCount {
   int share, sum;  // requests a lane, tiles up to the end of the lane's
+  Request last;    // the lane's last request
   __device__ __forceinline__ TileCount(const AttendArgs& a) {
     const int lane = threadIdx.x & 63;
     share = (a.n_seq + 63) / 64;
+    last = Request{0, 0, 0, 0};
     int mine = 0;
     for (int i = 0; i < share; ++i) {
       const int r = lane * share + i;
-      if (r < a.n_seq) mine += tiles_of<ROWS>(a, r);
+      if (r >= a.n_seq) break;
+      last = request_of(a, r);
+      mine += tiles_of<ROWS>(a, last);
     }
     sum = sum_up_to_lane(mine);
   }
   __device__ __forceinline__ int total() const { return __builtin_amdgcn_readlane(sum, 63); }
-  // The request of row tile `tile` < total(), and the tile's number in it.
-  __device__ __forceinline__ void find(const AttendArgs& a, int tile, int* request, int* local) const {
+  // The request of row tile `tile` < total(), its number, and the tile's in it.
+  __device__ __forceinline__ Request find(const AttendArgs& a, int tile, int* request, int* local) const {
     const int at = __builtin_ctzll(__ballot(sum > tile));  // the first lane whose share ends behind it
     int before = at ? __builtin_amdgcn_readlane(sum, at > 0 ? at - 1 : 0) : 0;
+    if (share == 1) {  // a lane holds what would be read again, which would be waited for
+      *request = at;
+      *local = tile - before;
+      return {__builtin_amdgcn_readlane(last.token0, at), __builtin_amdgcn_readlane(last.fresh, at),
+              __builtin_amdgcn_readlane(last.len, at), __builtin_amdgcn_readlane(last.keys, at)};
+    }
     for (int base = at * share;; base += 64) {
       const int r = base + static_cast<int>(threadIdx.x & 63);
-      const int up = sum_up_to_lane(r < a.n_seq && r < (at + 1) * share ? tiles_of<ROWS>(a, r) : 0);
+      const int up = sum_up_to_lane(r < a.n_seq && r < (at + 1) * share ? tiles_of<ROWS>(a, request_of(a, r)) : 0);
       const uint64_t behind = __ballot(before + up > tile);
       if (behind || base + 64 >= (at + 1) * share) {
         const int in = behind ? __builtin_ctzll(behind) : 0;
         *request = base + in;
         *local = tile - before - (in ? __builtin_amdgcn_readlane(up, in > 0 ? in - 1 : 0) : 0);
-        return;
+        return uniform_request_of(a, *request);
       }
       before += __builtin_amdgcn_readlane(up, 63);
     }
@@ -120,12 +127,11 @@ constexpr int kManyRounds = 6;
 struct ManyShares {
   int total, whole, splits;  // row tiles; those (the last ones) that are not split
   __device__ __forceinline__ ManyShares(const AttendArgs& a, const ManyGrid& grid, int tiles) : total(tiles), whole(tiles), splits(1) {
-    const int64_t items = static_cast<int64_t>(tiles) * a.kv_heads;
-    const int rounds = static_cast<int>(items / grid.round < kManyRounds ? items / grid.round : kManyRounds);
+    const int rounds = tiles * a.kv_heads / grid.round;  // fewer items than workgroups in the grid, below 2^31
     if (rounds >= kManyRounds) return;
-    const int left = tiles - static_cast<int>(static_cast<int64_t>(rounds) * grid.round / a.kv_heads);
+    const int left = tiles - rounds * grid.round / a.kv_heads;
     if (left <= 0) return;
-    const int fit = static_cast<int>(grid.round / (static_cast<int64_t>(left) * a.kv_heads));
+    const int fit = grid.round / (left * a.kv_heads);
     splits = fit < grid.most_splits ? fit : grid.most_splits;
     if (splits > 1)
       whole = tiles - left;
@@ -143,8 +149,8 @@ __global__ __launch_bounds__(ManyLayout<DP>::kThreads, ManyLayout<DP>::kGroups) 
   constexpr int kSteps = DP / 16;       // 16-dim steps of K Q^T
   constexpr int kBlocks = DP / 32;      // 32-dim blocks of the output
   constexpr int kKeyBlocks = L::kKeys / 32;
-  __shared__ __attribute__((aligned(16))) uint16_t k_tile[3][L::kTile];
-  __shared__ __attribute__((aligned(16))) uint16_t v_tile[3][L::kTile];
+  __shared__ __attribute__((aligned(16))) uint16_t k_tile[L::kBuffers][L::kTile];
+  __shared__ __attribute__((aligned(16))) uint16_t v_tile[L::kBuffers][L::kTile];
 
   // The last rows see the most keys: they begin first, and the ones that are
   // split end last.
@@ -159,8 +165,7 @@ __global__ __launch_bounds__(ManyLayout<DP>::kThreads, ManyLayout<DP>::kGroups) 
   const int tile = shares.total - 1 - (divided ? shares.whole + item : order);
   if (tile < 0) return;
   int request, local;
-  counted.find(a, tile, &request, &local);
-  const Request s = uniform_request_of(a, request);
+  const Request s = counted.find(a, tile, &request, &local);
   const int rows = s.fresh * a.qpk, row0 = local * kRows;
 
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
@@ -169,12 +174,12 @@ __global__ __launch_bounds__(ManyLayout<DP>::kThreads, ManyLayout<DP>::kGroups) 
   const int wg_last = (row0 + kRows < rows ? row0 + kRows : rows) - 1;
   const TileRange range = tile_range<L::kShift>(a, s, place0 + row0 / a.qpk, place0 + wg_last / a.qpk);
   const int count = range.count();
-  const int t_begin = static_cast<int>(static_cast<int64_t>(count) * split / splits);
-  const int t_end = static_cast<int>(static_cast<int64_t>(count) * (split + 1) / splits);
+  const int least = count / splits, more = count - least * splits;  // the first `more` splits take one tile more
+  const int t_begin = least * split + (split < more ? split : more);
+  const int t_end = t_begin + least + (split < more ? 1 : 0);
 
-  const int m = row0 + wave * 32 + col;
-  const bool inside = m < rows;
-  const int token = (inside ? m : rows - 1) / a.qpk, g = (inside ? m : rows - 1) - token * a.qpk;
+  const bool inside = row0 + wave * 32 + col < rows;
+  const int token = (inside ? row0 + wave * 32 + col : rows - 1) / a.qpk;
   RowSight sight = sight_of(a, s, place0 + token);
   if (!inside) sight.end = 0;
   // The wave's first and last rows' sights.
@@ -184,6 +189,7 @@ __global__ __launch_bounds__(ManyLayout<DP>::kThreads, ManyLayout<DP>::kGroups) 
 
   vec_t qf[kSteps];
   {
+    const int g = (inside ? row0 + wave * 32 + col : rows - 1) - token * a.qpk;
     const uint16_t* row = a.q + (s.token0 + token) * a.q_token_stride + (head * a.qpk + g) * a.q_head_stride;
 #pragma unroll
     for (int st = 0; st < kSteps; ++st) {
@@ -206,9 +212,6 @@ __global__ __launch_bounds__(ManyLayout<DP>::kThreads, ManyLayout<DP>::kGroups) 
   const int v_row = 4 * half + ((lane & 15) >> 2);
   const int v_from = v_row * L::kBytes + L::v_turn(v_row) + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
   u32x4 kst[L::kLoads], vst[L::kLoads];
-  // The queries are there before the first tile is asked for: the loop's waits
-  // then count its own loads alone.
-  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
   // A key tile's place in the pools and its bytes, up to the request's last row:
   // zeros come from behind it, whatever the page holds there, and for tiles behind
   // the last one or of pages outside the pool.  It is worked out in four steps of
@@ -229,6 +232,10 @@ __global__ __launch_bounds__(ManyLayout<DP>::kThreads, ManyLayout<DP>::kGroups) 
     const int block = t_end > 0 ? block_of(t) : 0;
     if (!pages.covers(block)) pages.refill(a, table, block);
   };
+  // The queries and the first pages are there before the first tile is asked for:
+  // the loop's waits then count its own loads alone.
+  pages.refill(a, table, t_end > 0 ? block_of(t_begin) : 0);
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
   auto seek = [&](Search& f, int t, int step) KVC_INLINE {
     if (step == 0) {
       f.key0 = range.tile(t < t_end ? t : (t_end > 0 ? t_end - 1 : 0)) << L::kShift;
@@ -285,21 +292,19 @@ __global__ __launch_bounds__(ManyLayout<DP>::kThreads, ManyLayout<DP>::kGroups) 
 #pragma unroll
   for (int b = 0; b < kBlocks; ++b) acc[b] = kZero;
   m_run = kNegInf;
-  l_run = 0.0f;
   // Weights of the tile before, and where its keys begin; none yet.
   vec_t pf[kKeyBlocks][2];
 #pragma unroll
   for (int kb = 0; kb < kKeyBlocks; ++kb) pf[kb][0] = pf[kb][1] = __builtin_bit_cast(vec_t, u32x4{0, 0, 0, 0});
   int key0 = 0;
-  f32x16 sc[kKeyBlocks];
-  float tops[4];
+  float tops[4], sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // in four chains: one would wait for itself
   // The products of a tile: S^T = K Q^T (if `scores`) from buffer `now`, then
   // O^T += V^T P^T of the tile before, from buffer `before`.  A left operand is
   // read kAhead products before its use, and the order is the source's (left to
   // itself the compiler reads one into the registers that the product before has
   // just freed, and each waits for LDS).  beside(i) is done between products.
   constexpr int kScores = kKeyBlocks * kSteps, kValues = kKeyBlocks * 2 * kBlocks;
-  constexpr int kAhead = L::kGroups > 1 ? 4 : 8;  // a second wave on the SIMD hides the rest
+  constexpr int kAhead = 4;
   vec_t ring[kAhead];
   auto k_operand = [&](int buffer, int i) KVC_INLINE {
     const char* at = reinterpret_cast<const char*>(k_tile[buffer]) + (k_from ^ (i / kKeyBlocks << 5)) + (i % kKeyBlocks) * 32 * L::kBytes;
@@ -309,7 +314,7 @@ __global__ __launch_bounds__(ManyLayout<DP>::kThreads, ManyLayout<DP>::kGroups) 
     const char* at = reinterpret_cast<const char*>(v_tile[buffer]) + (v_from ^ (i % kBlocks << 6)) + (i / kBlocks) * 16 * L::kBytes;
     return join_columns<vec_t>(read_column(at), read_column(at + 8 * L::kBytes));
   };
-  auto products = [&](auto scores, int now, int before, auto beside) KVC_INLINE {
+  auto products = [&](auto scores, f32x16 (&sc)[kKeyBlocks], int now, int before, auto beside) KVC_INLINE {
     constexpr int kFirst = decltype(scores)::value ? 0 : kScores, kAll = kScores + kValues;
     auto operand = [&](int i) { return i < kScores ? k_operand(now, i) : v_operand(before, i - kScores); };
     each<kFirst, kAll>([&](auto step) KVC_INLINE {
@@ -353,11 +358,122 @@ __global__ __launch_bounds__(ManyLayout<DP>::kThreads, ManyLayout<DP>::kGroups) 
     });
     __builtin_amdgcn_sched_barrier(0);
   };
-  // The maximum of a lane's scores, in four chains (one would wait for itself).
-  auto top_of = [&](int e) KVC_INLINE { tops[e & 3] = fmaxf(tops[e & 3], sc[e >> 4][e & 15]); };
+  // The maximum of a lane's scores.
+  auto top_of = [&](const f32x16 (&sc)[kKeyBlocks], int e) KVC_INLINE { tops[e & 3] = fmaxf(tops[e & 3], sc[e >> 4][e & 15]); };
   auto all_tops = [&]() KVC_INLINE { return max_across_halves(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]))); };
   constexpr int kLane = kKeyBlocks * 16;  // scores of a lane
+  // The softmax of the scores in `sc`, whose maximum is `top`: masks and the
+  // maximum, then the weights two by two, in `pf`.
+  float m_use;
+  // With one group a SIMD has 512 registers a wave, half of them for the matrix
+  // products alone.  The outputs stay in those (left to itself the compiler moves
+  // them out for the rare scaling and back at every tile).
+  auto hold = [&]() KVC_INLINE {
+    if constexpr (L::kGroups == 1) {
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) asm volatile("" : "+a"(acc[b]));
+    }
+  };
+  auto prepare = [&](f32x16 (&sc)[kKeyBlocks], float top) KVC_INLINE {
+    if (!(key0 + L::kKeys <= first.end && (key0 >= last.low || key0 + L::kKeys <= a.sinks))) {
+      tops[0] = tops[1] = tops[2] = tops[3] = kNegInf;
+#pragma unroll
+      for (int e = 0; e < kLane; ++e) {
+        const int i = e & 15;
+        sc[e >> 4][i] = sees(sight, a.sinks, key0 + (e >> 4) * 32 + 8 * (i >> 2) + 4 * half + (i & 3)) ? sc[e >> 4][i] : kNegInf;
+        top_of(sc, e);
+      }
+      top = all_tops();
+    }
+    top *= a.scale_log2;
+    // The maximum moves only when it grows by more than 2^8: weights then reach
+    // 2^8 at most, and most tiles leave the outputs unscaled.
+    const float m_new = top > m_run + 8.0f ? top : m_run;
+    if (__any(m_new != m_run)) {
+      const float scale = m_new == kNegInf ? 1.0f : exp2_fast(m_run - m_new);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sums[i] *= scale;
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) acc[b] *= scale;
+      m_run = m_new;
+      hold();
+    }
+    m_use = m_run == kNegInf ? 0.0f : m_run;
+  };
+  auto weigh = [&](const f32x16 (&sc)[kKeyBlocks], int e) KVC_INLINE {
+    const int kb = e >> 4, i = e & 15;
+    const float p0 = exp2_fast(fmaf(sc[kb][i], a.scale_log2, -m_use)), p1 = exp2_fast(fmaf(sc[kb][i + 1], a.scale_log2, -m_use));
+    sums[i >> 1 & 3] += p0 + p1;
+    u32x4 w = __builtin_bit_cast(u32x4, pf[kb][i >> 3]);
+    w[i >> 1 & 3] = E::pack(p0, p1);
+    pf[kb][i >> 3] = __builtin_bit_cast(vec_t, w);
+  };
 
+  if constexpr (L::kGroups == 1) {
+    // One group: a tile's weights are formed beside the scores' products of the
+    // next one.
+    load(a.k, place_of(t_begin), kst);
+    load(a.v, place_of(t_begin), vst);
+    uint32_t there = place_of(t_begin).bytes != 0;  // whether the tiles from t on are in the pool, t lowest
+    store_k(0);
+    store_v(0);
+    Place ahead = place_of(t_begin + 1);
+    there |= static_cast<uint32_t>(ahead.bytes != 0) << 1;
+    load(a.k, ahead, kst);
+    load(a.v, ahead, vst);
+    store_k(1);
+    ahead = place_of(t_begin + 2);  // of tile t + 2
+    there |= static_cast<uint32_t>(ahead.bytes != 0) << 2;
+    load(a.k, ahead, kst);
+    ready(t_begin + 3);
+    __syncthreads();
+    f32x16 sc[2][kKeyBlocks];
+#pragma unroll
+    for (int i = 0; i < kScores; ++i) {
+      const int kb = i % kKeyBlocks, st = i / kKeyBlocks;
+      sc[0][kb] = E::mfma32(k_operand(0, i), qf[st], st ? sc[0][kb] : kZero);
+    }
+    tops[0] = tops[1] = tops[2] = tops[3] = kNegInf;
+#pragma unroll
+    for (int e = 0; e < kLane; ++e) top_of(sc[0], e);
+    float top = all_tops();
+    __syncthreads();
+    auto turn = [&](auto parity, int t) KVC_INLINE {
+      constexpr int own = decltype(parity)::value, other = 1 - own;  // of tile t and t + 1: buffers, scores
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) ring[i] = k_operand(other, i);
+      // No key of a page outside the pool is seen: its tile lies behind every row.
+      key0 = there & 1 ? range.tile(t) << L::kShift : 1 << 30;
+      hold();
+      prepare(sc[own], top);
+      Search search;
+      tops[0] = tops[1] = tops[2] = tops[3] = kNegInf;
+      products(std::true_type{}, sc[other], other, own, [&](int i) KVC_INLINE {
+#pragma unroll
+        for (int e = 0; e < kLane; e += 2)
+          if (i == e / 2 * kScores / (kLane / 2)) weigh(sc[own], e);
+        if (i == 1) store_k(own);    // tile t + 2; tile t's K was last read a barrier ago
+        if (i == 3) store_v(other);  // tile t + 1
+        if (i >= 4 && i < 8) seek(search, t + 3, i - 4);
+        if (i == 8) load(a.v, ahead, vst);
+        if (i == 9) load(a.k, search.at, kst);
+        constexpr int kFrom = kScores + 2, kTo = kScores + kValues;  // the scores are there
+#pragma unroll
+        for (int e = 0; e < kLane; ++e)
+          if (i == kFrom + e / 2 * 2 * (kTo - kFrom) / kLane) top_of(sc[other], e);
+        if (i == kTo - 1) top = all_tops();
+      });
+      ahead = search.at;
+      there = there >> 1 | static_cast<uint32_t>(search.at.bytes != 0) << 2;
+      ready(t + 4);
+      __syncthreads();
+    };
+    for (int t = t_begin; t < t_end; t += 2) {
+      turn(std::integral_constant<int, 0>{}, t);
+      turn(std::integral_constant<int, 1>{}, t + 1);  // no key of a tile behind the last one is seen
+    }
+  } else {
+  f32x16 sc[kKeyBlocks];
   // The first tile of K, a tile of zeros as V before it, and what the second group
   // stores ahead; the next ones wait in registers.
   int now = 0, next = 1, before = 2;  // buffers of tiles t, t + 1 and t - 1
@@ -394,7 +510,7 @@ __global__ __launch_bounds__(ManyLayout<DP>::kThreads, ManyLayout<DP>::kGroups) 
     float top;
     tops[0] = tops[1] = tops[2] = tops[3] = kNegInf;
     __builtin_amdgcn_s_setprio(1);
-    products(std::true_type{}, now, before, [&](int i) KVC_INLINE {
+    products(std::true_type{}, sc, now, before, [&](int i) KVC_INLINE {
       if (i == 1) store_k(group ? before : next);
       if (i == 2) store_v(group ? next : now);
       if (i >= 3 && i < 7) seek(search, t + 2 + group, i - 3);
@@ -403,7 +519,7 @@ __global__ __launch_bounds__(ManyLayout<DP>::kThreads, ManyLayout<DP>::kGroups) 
       constexpr int kFrom = kScores + 2, kTo = kScores + kValues;  // the scores are there
 #pragma unroll
       for (int e = 0; e < kLane; ++e)
-        if (i == kFrom + e / 2 * 2 * (kTo - kFrom) / kLane) top_of(e);
+        if (i == kFrom + e / 2 * 2 * (kTo - kFrom) / kLane) top_of(sc, e);
       if (i == kTo - 1) top = all_tops();
     });
     __builtin_amdgcn_s_setprio(0);
@@ -414,44 +530,9 @@ __global__ __launch_bounds__(ManyLayout<DP>::kThreads, ManyLayout<DP>::kGroups) 
     __syncthreads();
     __builtin_amdgcn_sched_barrier(0);
     // Softmax.
-    if (!(key0 + L::kKeys <= first.end && (key0 >= last.low || key0 + L::kKeys <= a.sinks))) {
-      tops[0] = tops[1] = tops[2] = tops[3] = kNegInf;
+    prepare(sc, top);
 #pragma unroll
-      for (int e = 0; e < kLane; ++e) {
-        const int i = e & 15;
-        sc[e >> 4][i] = sees(sight, a.sinks, key0 + (e >> 4) * 32 + 8 * (i >> 2) + 4 * half + (i & 3)) ? sc[e >> 4][i] : kNegInf;
-        top_of(e);
-      }
-      top = all_tops();
-    }
-    top *= a.scale_log2;
-    // The maximum moves only when it grows by more than 2^8: weights then reach
-    // 2^8 at most, and most tiles leave the outputs unscaled.
-    const float m_new = top > m_run + 8.0f ? top : m_run;
-    if (__any(m_new != m_run)) {
-      const float scale = m_new == kNegInf ? 1.0f : exp2_fast(m_run - m_new);
-      l_run *= scale;
-#pragma unroll
-      for (int b = 0; b < kBlocks; ++b) acc[b] *= scale;
-      m_run = m_new;
-    }
-    const float m_use = m_run == kNegInf ? 0.0f : m_run;
-    float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int kb = 0; kb < kKeyBlocks; ++kb)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        u32x4 w;
-#pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-          const float p0 = exp2_fast(fmaf(sc[kb][8 * h + j], a.scale_log2, -m_use));
-          const float p1 = exp2_fast(fmaf(sc[kb][8 * h + j + 1], a.scale_log2, -m_use));
-          sums[j >> 1] += p0 + p1;
-          w[j >> 1] = E::pack(p0, p1);
-        }
-        pf[kb][h] = __builtin_bit_cast(vec_t, w);
-      }
-    l_run += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    for (int e = 0; e < kLane; e += 2) weigh(sc, e);
     ready(t + 3 + group);
     // The next products' first operands: they have been there for a phase.
     const int free = before;
@@ -469,8 +550,10 @@ __global__ __launch_bounds__(ManyLayout<DP>::kThreads, ManyLayout<DP>::kGroups) 
   }
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) ring[i] = v_operand(before, i);
-  products(std::false_type{}, now, before, [](int) {});
-  if (L::kGroups > 1 && !group) __syncthreads();
+  products(std::false_type{}, sc, now, before, [](int) {});
+  if (!group) __syncthreads();
+  }
+  l_run = (sums[0] + sums[1]) + (sums[2] + sums[3]);
   bool wild = false;
 #pragma unroll
   for (int b = 0; b < kBlocks; ++b)
@@ -481,9 +564,13 @@ __global__ __launch_bounds__(ManyLayout<DP>::kThreads, ManyLayout<DP>::kGroups) 
   if (__syncthreads_or(go_over(std::false_type{}))) go_over(std::true_type{});
 
   const float l_all = l_run + __shfl_xor(l_run, 32);
-  if (!inside) return;
+  int thread = tid;
+  asm volatile("" : "+v"(thread));  // the row's place is worked out anew, not held through the loop
+  const int local_row = (thread >> 6) * 32 + (thread & 31), m = row0 + local_row;
+  if (m >= rows) return;
   if (!divided) {
     const float inv = l_all == 0.0f ? 0.0f : 1.0f / l_all;
+    const int token = m / a.qpk, g = m - token * a.qpk;
     uint16_t* to = a.out + (s.token0 + token) * a.out_token_stride + (head * a.qpk + g) * a.out_head_stride;
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b)
@@ -496,14 +583,13 @@ __global__ __launch_bounds__(ManyLayout<DP>::kThreads, ManyLayout<DP>::kGroups) 
       }
   } else {
     float* const piece = a.partial + ((static_cast<int64_t>(item) * a.kv_heads + head) * splits + split) * piece_floats(kRows, DP);
-    const int local = m - row0;
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        *gptr(reinterpret_cast<f32x4*>(piece + local * DP + b * 32 + i * 8 + half * 4)) =
+        *gptr(reinterpret_cast<f32x4*>(piece + local_row * DP + b * 32 + i * 8 + half * 4)) =
             f32x4{acc[b][4 * i], acc[b][4 * i + 1], acc[b][4 * i + 2], acc[b][4 * i + 3]};
-    if (half == 0) *gptr(reinterpret_cast<f32x2*>(piece + kRows * DP + 2 * local)) = f32x2{m_run, l_all};
+    if (half == 0) *gptr(reinterpret_cast<f32x2*>(piece + kRows * DP + 2 * local_row)) = f32x2{m_run, l_all};
   }
 }
 
@@ -518,8 +604,7 @@ __global__ __launch_bounds__(kJoinThreads) void attend_many_join_kernel(AttendAr
   const int tile = shares.total - 1 - shares.whole - item;
   if (tile < 0) return;
   int request, local_tile;
-  counted.find(a, tile, &request, &local_tile);
-  const Request s = uniform_request_of(a, request);
+  const Request s = counted.find(a, tile, &request, &local_tile);
   const int row0 = local_tile * kRows, left = s.fresh * a.qpk - row0;
   const int64_t size = piece_floats(kRows, DP);
   const float* const pieces = a.partial + (static_cast<int64_t>(item) * a.kv_heads + head) * shares.splits * size;
