@@ -280,6 +280,26 @@ def test_attend_random_shapes(hip_device, seed) -> None:
     _check(got, q, caches[:2], start, lens, caches[2], dtype, scale=0.3, window=window, sinks=sinks, rows_most=max(new) * heads // kv)
 
 
+@pytest.mark.parametrize("window, sinks", [(0, 0), (100, 5)])
+@pytest.mark.parametrize("heads, kv, dim, dtype", [
+    (16, 8, 64, BF16), (24, 8, 96, FP16), (40, 8, 128, BF16), (8, 8, 192, BF16), (16, 8, 192, FP16), (16, 8, 256, BF16), (64, 8, 256, BF16),
+])
+def test_attend_short_requests_apart_from_chunks(hip_device, heads, kv, dim, dtype, window, sinks) -> None:
+    """A table so wide that short requests and chunks get a launch each, and a
+    narrow one that gives them one: both are the definition's values."""
+    g = torch.Generator().manual_seed(dim + heads)
+    lens, new = [700, 1, 300, 2100, 5, 0], [2, 1, 150, 1, 5, 0]
+    start = [0, *torch.tensor(new).cumsum(0).tolist()]
+    q = torch.randn((start[-1], heads, dim), generator=g).to(dtype)
+    d = lambda x: torch.tensor(x, dtype=torch.int32, device=hip_device)  # noqa: E731
+    for width in (600, 20):
+        caches = _paged(lens, kv, dim, dtype, torch.Generator().manual_seed(dim), max_blocks=width)
+        got = _serving().attend_paged(q.to(hip_device), caches[0].to(hip_device), caches[1].to(hip_device), d(start), d(lens),
+                                      caches[2].to(hip_device), max_query_len=max(new), window=window, sinks=sinks)
+        _check(got, q, caches[:2], start, lens, caches[2], dtype, scale=dim**-0.5, window=window, sinks=sinks,
+               rows_most=max(new) * heads // kv)
+
+
 @pytest.mark.parametrize("dim, dtype", [(128, BF16), (128, FP16), (256, BF16), (96, BF16)])
 @pytest.mark.parametrize("new, window, sinks", [(3, 0, 0), (4, 7, 2), (60, 0, 0), (60, 9, 1)])
 def test_hidden_values_reach_no_row_that_does_not_see_them(hip_device, dim, dtype, new, window, sinks) -> None:
@@ -401,7 +421,7 @@ def test_attend_more_requests_than_one_launch_takes(hip_device) -> None:
     q = torch.randn((n, 2, dim), generator=g, device=hip_device).to(BF16)
     start = torch.arange(n + 1, dtype=torch.int32, device=hip_device)
     got = _serving().attend_paged(q, pool[0], pool[1], start, lens, table, max_query_len=1)
-    for r in (0, 2047, 2048, 4095, 4096, 4999):
+    for r in (0, 1023, 1024, 2047, 2048, 4095, 4096, 4999):
         one = _serving().attend_paged(q[r : r + 1], pool[0], pool[1], start[:2], lens[r : r + 1], table[r : r + 1])
         torch.testing.assert_close(got[r : r + 1], one, rtol=2.0**-7, atol=2.0**-12)
 

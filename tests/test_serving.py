@@ -196,6 +196,7 @@ def _attend_c(lib, **change):
     ({"tokens": 1 << 24}, "bad sizes"),
     ({"page": 128 * 2 * 128 - 8}, "page_stride"),
     ({"page": 128 * 2 * 128 + 4}, "page_stride"),
+    ({"page": 1 << 31}, "page_stride"),
     ({"blocks": 5}, "block_table_stride"),
     ({"blocks": 1 << 23, "stride": 1 << 23}, "max_blocks"),
     ({"scale": -1.0}, "scale"),

@@ -266,7 +266,7 @@ constexpr int kFewRows = 16;         // rows of one few-rows tile
 constexpr int kFewTilesMost = 2;     // tiles of a request that the few-rows kernel takes
 constexpr int kFewSequences = 1024;  // requests of one launch (their prefix sums sit in LDS)
 // Rows of one many-rows tile, 32 a wave.
-constexpr int many_rows(int dim) { return dim <= 128 ? 256 : 128; }
+constexpr int many_rows(int dim) { return dim <= 192 ? 256 : 128; }
 
 // Few-rows workgroups that a compute unit holds.
 constexpr int few_residents(int dim) { return dim <= 64 ? 3 : (dim <= 128 ? 2 : 1); }
