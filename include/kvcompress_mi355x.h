@@ -457,9 +457,11 @@ int kvc_rotate_and_store(kvc_stream_t stream, int dtype, int rope_style, int64_t
  * multiple of 8 up to 256.  max_query_len must bound every request's new tokens
  * (rows of longer ones may be left out); max_seq_len sizes the launch only.
  * scale is positive.  out may not overlap q; its rows outside every request are
- * left as they were.  Scores, softmax and sums are float32; the weights of
- * requests with more than 32 rows (new*qpk) are rounded to the cache's type
- * before the product with V.  Results are the same on every run of a shape.
+ * left as they were.  Scores, softmax and sums are float32; where max_query_len *
+ * qpk is more than 32, weights may be rounded to the cache's type before the
+ * product with V (half a step of it), else they keep twice its bits.  Results are
+ * the same on every run with the same arguments.  page_stride below 2^31 elements,
+ * max_blocks below 2^23, kv_heads * max_blocks at most 2^30.
  * workspace: kvc_attend_workspace_bytes of the same sizes (0 for sizes that are
  * refused), any contents; calls that overlap in time need one each.
  * No counterpart in the reference (its host's attention backend reads the cache). */

@@ -1,9 +1,22 @@
 // Attention of requests with many rows (chunks of a prompt): the matrix cores
-// bound it.  A workgroup takes 128 rows of one (request, KV head), 32 a wave,
-// and walks the key tiles that some row sees; K and V tiles pass through LDS,
-// two buffers deep, the next tile's loads in registers while one is worked on.
-// With few tiles of rows the keys are split too, and a second launch joins the
-// splits.
+// bound it.  A workgroup takes 128 or 256 rows of one (request, KV head), 32 a
+// wave, and walks the key tiles that some row sees; K and V tiles go through
+// registers to LDS, where all waves read them.  With few tiles of rows the keys
+// are split too, and a second launch joins the splits.
+//
+// What runs beside the matrix products is what decides.  Up to head_dim 192 two
+// waves share a SIMD: two groups of four waves take 128 rows each, the second
+// half a tile behind the first, so that one's products run beside the other's
+// softmax.  Above that a wave's outputs and queries need more registers than half
+// a SIMD's: one group forms a tile's weights between the products of the next
+// tile's scores.
+//
+// 2048 tokens (40 heads on 8, head_dim 128) over 16384 keys: 600 us, 1.07
+// PFLOP/s, a library product of 16384^3 1.58.  There the card's power is the
+// limit: the kernel needs 1.19 million cycles at 1.93 GHz, its simpler forms
+// 1.48 million at 2.19 GHz took hardly longer.  16 heads on 2: head_dim 64 311 us
+// of 4096 tokens (0.9 PFLOP/s, the softmax's), of 2048 head_dim 192 403 us (1.0)
+// and 256 593 us (0.9).
 //
 // Scores are formed transposed (S^T = K Q^T, 32x32x16): a lane holds one row's
 // scores (its other half in lane ^ 32), so the softmax needs one exchange, and
@@ -288,278 +301,278 @@ __global__ __launch_bounds__(ManyLayout<DP>::kThreads, ManyLayout<DP>::kGroups) 
   // not see it.  That shows in the outputs: a workgroup that finds one there
   // goes over its keys again with care.  Returns whether the thread has one.
   auto go_over = [&](auto care) KVC_INLINE {
-  constexpr bool careful = decltype(care)::value;
+    constexpr bool careful = decltype(care)::value;
 #pragma unroll
-  for (int b = 0; b < kBlocks; ++b) acc[b] = kZero;
-  m_run = kNegInf;
-  // Weights of the tile before, and where its keys begin; none yet.
-  vec_t pf[kKeyBlocks][2];
+    for (int b = 0; b < kBlocks; ++b) acc[b] = kZero;
+    m_run = kNegInf;
+    // Weights of the tile before, and where its keys begin; none yet.
+    vec_t pf[kKeyBlocks][2];
 #pragma unroll
-  for (int kb = 0; kb < kKeyBlocks; ++kb) pf[kb][0] = pf[kb][1] = __builtin_bit_cast(vec_t, u32x4{0, 0, 0, 0});
-  int key0 = 0;
-  float tops[4], sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // in four chains: one would wait for itself
-  // The products of a tile: S^T = K Q^T (if `scores`) from buffer `now`, then
-  // O^T += V^T P^T of the tile before, from buffer `before`.  A left operand is
-  // read kAhead products before its use, and the order is the source's (left to
-  // itself the compiler reads one into the registers that the product before has
-  // just freed, and each waits for LDS).  beside(i) is done between products.
-  constexpr int kScores = kKeyBlocks * kSteps, kValues = kKeyBlocks * 2 * kBlocks;
-  constexpr int kAhead = 4;
-  vec_t ring[kAhead];
-  auto k_operand = [&](int buffer, int i) KVC_INLINE {
-    const char* at = reinterpret_cast<const char*>(k_tile[buffer]) + (k_from ^ (i / kKeyBlocks << 5)) + (i % kKeyBlocks) * 32 * L::kBytes;
-    return __builtin_bit_cast(vec_t, *reinterpret_cast<const u32x4*>(at));
-  };
-  auto v_operand = [&](int buffer, int i) KVC_INLINE {
-    const char* at = reinterpret_cast<const char*>(v_tile[buffer]) + (v_from ^ (i % kBlocks << 6)) + (i / kBlocks) * 16 * L::kBytes;
-    return join_columns<vec_t>(read_column(at), read_column(at + 8 * L::kBytes));
-  };
-  auto products = [&](auto scores, f32x16 (&sc)[kKeyBlocks], int now, int before, auto beside) KVC_INLINE {
-    constexpr int kFirst = decltype(scores)::value ? 0 : kScores, kAll = kScores + kValues;
-    auto operand = [&](int i) { return i < kScores ? k_operand(now, i) : v_operand(before, i - kScores); };
-    each<kFirst, kAll>([&](auto step) KVC_INLINE {
-      constexpr int i = decltype(step)::value;
-      __builtin_amdgcn_sched_barrier(0);
-      vec_t left = ring[(i - kFirst) % kAhead];
-      if constexpr (i < kScores) {
-        const int kb = i % kKeyBlocks, st = i / kKeyBlocks;
-        sc[kb] = E::mfma32(left, qf[st], st ? sc[kb] : kZero);
-      } else {
-        const int b = (i - kScores) % kBlocks, kh = (i - kScores) / kBlocks, kb = kh >> 1, h = kh & 1;
-        if constexpr (careful) {
-          // Values that are not finite are added only to the rows that see them,
-          // token by token.
-          s16x8 raw = __builtin_bit_cast(s16x8, left), odd = {0, 0, 0, 0, 0, 0, 0, 0};
-          bool any = false;
+    for (int kb = 0; kb < kKeyBlocks; ++kb) pf[kb][0] = pf[kb][1] = __builtin_bit_cast(vec_t, u32x4{0, 0, 0, 0});
+    int key0 = 0;
+    float tops[4], sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // in four chains: one would wait for itself
+    // The products of a tile: S^T = K Q^T (if `scores`) from buffer `now`, then
+    // O^T += V^T P^T of the tile before, from buffer `before`.  A left operand is
+    // read kAhead products before its use, and the order is the source's (left to
+    // itself the compiler reads one into the registers that the product before has
+    // just freed, and each waits for LDS).  beside(i) is done between products.
+    constexpr int kScores = kKeyBlocks * kSteps, kValues = kKeyBlocks * 2 * kBlocks;
+    constexpr int kAhead = 4;  // 6 to 12 are 2 to 7% slower at head_dim 256, one group's
+    vec_t ring[kAhead];
+    auto k_operand = [&](int buffer, int i) KVC_INLINE {
+      const char* at = reinterpret_cast<const char*>(k_tile[buffer]) + (k_from ^ (i / kKeyBlocks << 5)) + (i % kKeyBlocks) * 32 * L::kBytes;
+      return __builtin_bit_cast(vec_t, *reinterpret_cast<const u32x4*>(at));
+    };
+    auto v_operand = [&](int buffer, int i) KVC_INLINE {
+      const char* at = reinterpret_cast<const char*>(v_tile[buffer]) + (v_from ^ (i % kBlocks << 6)) + (i / kBlocks) * 16 * L::kBytes;
+      return join_columns<vec_t>(read_column(at), read_column(at + 8 * L::kBytes));
+    };
+    auto products = [&](auto scores, f32x16 (&sc)[kKeyBlocks], int now, int before, auto beside) KVC_INLINE {
+      constexpr int kFirst = decltype(scores)::value ? 0 : kScores, kAll = kScores + kValues;
+      auto operand = [&](int i) { return i < kScores ? k_operand(now, i) : v_operand(before, i - kScores); };
+      each<kFirst, kAll>([&](auto step) KVC_INLINE {
+        constexpr int i = decltype(step)::value;
+        __builtin_amdgcn_sched_barrier(0);
+        vec_t left = ring[(i - kFirst) % kAhead];
+        if constexpr (i < kScores) {
+          const int kb = i % kKeyBlocks, st = i / kKeyBlocks;
+          sc[kb] = E::mfma32(left, qf[st], st ? sc[kb] : kZero);
+        } else {
+          const int b = (i - kScores) % kBlocks, kh = (i - kScores) / kBlocks, kb = kh >> 1, h = kh & 1;
+          if constexpr (careful) {
+            // Values that are not finite are added only to the rows that see them,
+            // token by token.
+            s16x8 raw = __builtin_bit_cast(s16x8, left), odd = {0, 0, 0, 0, 0, 0, 0, 0};
+            bool any = false;
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if ((static_cast<uint16_t>(raw[j]) & E::kExponent) == E::kExponent) {
-              odd[j] = raw[j];
-              raw[j] = 0;
-              any = true;
-            }
-          left = __builtin_bit_cast(vec_t, raw);
-          if (__any(any)) {
-            for (int n = token_first; n <= token_last; ++n) {
-              const RowSight one = sight_of(a, s, place0 + n);
-              s16x8 seen = odd;
+            for (int j = 0; j < 8; ++j)
+              if ((static_cast<uint16_t>(raw[j]) & E::kExponent) == E::kExponent) {
+                odd[j] = raw[j];
+                raw[j] = 0;
+                any = true;
+              }
+            left = __builtin_bit_cast(vec_t, raw);
+            if (__any(any)) {
+              for (int n = token_first; n <= token_last; ++n) {
+                const RowSight one = sight_of(a, s, place0 + n);
+                s16x8 seen = odd;
 #pragma unroll
-              for (int j = 0; j < 8; ++j)
-                if (!sees(one, a.sinks, key0 + kb * 32 + h * 16 + 8 * (j >> 2) + 4 * half + (j & 3))) seen[j] = 0;
-              const f32x16 more = E::mfma32(__builtin_bit_cast(vec_t, seen), pf[kb][h], kZero);
-              if (token == n) acc[b] += more;
+                for (int j = 0; j < 8; ++j)
+                  if (!sees(one, a.sinks, key0 + kb * 32 + h * 16 + 8 * (j >> 2) + 4 * half + (j & 3))) seen[j] = 0;
+                const f32x16 more = E::mfma32(__builtin_bit_cast(vec_t, seen), pf[kb][h], kZero);
+                if (token == n) acc[b] += more;
+              }
             }
           }
+          acc[b] = E::mfma32(left, pf[kb][h], acc[b]);
         }
-        acc[b] = E::mfma32(left, pf[kb][h], acc[b]);
-      }
-      if (i + kAhead < kAll) ring[(i - kFirst) % kAhead] = operand(i + kAhead);
-      beside(i);
-    });
-    __builtin_amdgcn_sched_barrier(0);
-  };
-  // The maximum of a lane's scores.
-  auto top_of = [&](const f32x16 (&sc)[kKeyBlocks], int e) KVC_INLINE { tops[e & 3] = fmaxf(tops[e & 3], sc[e >> 4][e & 15]); };
-  auto all_tops = [&]() KVC_INLINE { return max_across_halves(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]))); };
-  constexpr int kLane = kKeyBlocks * 16;  // scores of a lane
-  // The softmax of the scores in `sc`, whose maximum is `top`: masks and the
-  // maximum, then the weights two by two, in `pf`.
-  float m_use;
-  // With one group a SIMD has 512 registers a wave, half of them for the matrix
-  // products alone.  The outputs stay in those (left to itself the compiler moves
-  // them out for the rare scaling and back at every tile).
-  auto hold = [&]() KVC_INLINE {
-    if constexpr (L::kGroups == 1) {
-#pragma unroll
-      for (int b = 0; b < kBlocks; ++b) asm volatile("" : "+a"(acc[b]));
-    }
-  };
-  auto prepare = [&](f32x16 (&sc)[kKeyBlocks], float top) KVC_INLINE {
-    if (!(key0 + L::kKeys <= first.end && (key0 >= last.low || key0 + L::kKeys <= a.sinks))) {
-      tops[0] = tops[1] = tops[2] = tops[3] = kNegInf;
-#pragma unroll
-      for (int e = 0; e < kLane; ++e) {
-        const int i = e & 15;
-        sc[e >> 4][i] = sees(sight, a.sinks, key0 + (e >> 4) * 32 + 8 * (i >> 2) + 4 * half + (i & 3)) ? sc[e >> 4][i] : kNegInf;
-        top_of(sc, e);
-      }
-      top = all_tops();
-    }
-    top *= a.scale_log2;
-    // The maximum moves only when it grows by more than 2^8: weights then reach
-    // 2^8 at most, and most tiles leave the outputs unscaled.
-    const float m_new = top > m_run + 8.0f ? top : m_run;
-    if (__any(m_new != m_run)) {
-      const float scale = m_new == kNegInf ? 1.0f : exp2_fast(m_run - m_new);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sums[i] *= scale;
-#pragma unroll
-      for (int b = 0; b < kBlocks; ++b) acc[b] *= scale;
-      m_run = m_new;
-      hold();
-    }
-    m_use = m_run == kNegInf ? 0.0f : m_run;
-  };
-  auto weigh = [&](const f32x16 (&sc)[kKeyBlocks], int e) KVC_INLINE {
-    const int kb = e >> 4, i = e & 15;
-    const float p0 = exp2_fast(fmaf(sc[kb][i], a.scale_log2, -m_use)), p1 = exp2_fast(fmaf(sc[kb][i + 1], a.scale_log2, -m_use));
-    sums[i >> 1 & 3] += p0 + p1;
-    u32x4 w = __builtin_bit_cast(u32x4, pf[kb][i >> 3]);
-    w[i >> 1 & 3] = E::pack(p0, p1);
-    pf[kb][i >> 3] = __builtin_bit_cast(vec_t, w);
-  };
-
-  if constexpr (L::kGroups == 1) {
-    // One group: a tile's weights are formed beside the scores' products of the
-    // next one.
-    load(a.k, place_of(t_begin), kst);
-    load(a.v, place_of(t_begin), vst);
-    uint32_t there = place_of(t_begin).bytes != 0;  // whether the tiles from t on are in the pool, t lowest
-    store_k(0);
-    store_v(0);
-    Place ahead = place_of(t_begin + 1);
-    there |= static_cast<uint32_t>(ahead.bytes != 0) << 1;
-    load(a.k, ahead, kst);
-    load(a.v, ahead, vst);
-    store_k(1);
-    ahead = place_of(t_begin + 2);  // of tile t + 2
-    there |= static_cast<uint32_t>(ahead.bytes != 0) << 2;
-    load(a.k, ahead, kst);
-    ready(t_begin + 3);
-    __syncthreads();
-    f32x16 sc[2][kKeyBlocks];
-#pragma unroll
-    for (int i = 0; i < kScores; ++i) {
-      const int kb = i % kKeyBlocks, st = i / kKeyBlocks;
-      sc[0][kb] = E::mfma32(k_operand(0, i), qf[st], st ? sc[0][kb] : kZero);
-    }
-    tops[0] = tops[1] = tops[2] = tops[3] = kNegInf;
-#pragma unroll
-    for (int e = 0; e < kLane; ++e) top_of(sc[0], e);
-    float top = all_tops();
-    __syncthreads();
-    auto turn = [&](auto parity, int t) KVC_INLINE {
-      constexpr int own = decltype(parity)::value, other = 1 - own;  // of tile t and t + 1: buffers, scores
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) ring[i] = k_operand(other, i);
-      // No key of a page outside the pool is seen: its tile lies behind every row.
-      key0 = there & 1 ? range.tile(t) << L::kShift : 1 << 30;
-      hold();
-      prepare(sc[own], top);
-      Search search;
-      tops[0] = tops[1] = tops[2] = tops[3] = kNegInf;
-      products(std::true_type{}, sc[other], other, own, [&](int i) KVC_INLINE {
-#pragma unroll
-        for (int e = 0; e < kLane; e += 2)
-          if (i == e / 2 * kScores / (kLane / 2)) weigh(sc[own], e);
-        if (i == 1) store_k(own);    // tile t + 2; tile t's K was last read a barrier ago
-        if (i == 3) store_v(other);  // tile t + 1
-        if (i >= 4 && i < 8) seek(search, t + 3, i - 4);
-        if (i == 8) load(a.v, ahead, vst);
-        if (i == 9) load(a.k, search.at, kst);
-        constexpr int kFrom = kScores + 2, kTo = kScores + kValues;  // the scores are there
-#pragma unroll
-        for (int e = 0; e < kLane; ++e)
-          if (i == kFrom + e / 2 * 2 * (kTo - kFrom) / kLane) top_of(sc[other], e);
-        if (i == kTo - 1) top = all_tops();
+        if (i + kAhead < kAll) ring[(i - kFirst) % kAhead] = operand(i + kAhead);
+        beside(i);
       });
-      ahead = search.at;
-      there = there >> 1 | static_cast<uint32_t>(search.at.bytes != 0) << 2;
-      ready(t + 4);
-      __syncthreads();
+      __builtin_amdgcn_sched_barrier(0);
     };
-    for (int t = t_begin; t < t_end; t += 2) {
-      turn(std::integral_constant<int, 0>{}, t);
-      turn(std::integral_constant<int, 1>{}, t + 1);  // no key of a tile behind the last one is seen
+    // The maximum of a lane's scores.
+    auto top_of = [&](const f32x16 (&sc)[kKeyBlocks], int e) KVC_INLINE { tops[e & 3] = fmaxf(tops[e & 3], sc[e >> 4][e & 15]); };
+    auto all_tops = [&]() KVC_INLINE { return max_across_halves(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]))); };
+    constexpr int kLane = kKeyBlocks * 16;  // scores of a lane
+    // The softmax of the scores in `sc`, whose maximum is `top`: masks and the
+    // maximum, then the weights two by two, in `pf`.
+    float m_use;
+    // With one group a SIMD has 512 registers a wave, half of them for the matrix
+    // products alone.  The outputs stay in those (left to itself the compiler moves
+    // them out for the rare scaling and back at every tile).
+    auto hold = [&]() KVC_INLINE {
+      if constexpr (L::kGroups == 1) {
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) asm volatile("" : "+a"(acc[b]));
+      }
+    };
+    auto prepare = [&](f32x16 (&sc)[kKeyBlocks], float top) KVC_INLINE {
+      if (!(key0 + L::kKeys <= first.end && (key0 >= last.low || key0 + L::kKeys <= a.sinks))) {
+        tops[0] = tops[1] = tops[2] = tops[3] = kNegInf;
+#pragma unroll
+        for (int e = 0; e < kLane; ++e) {
+          const int i = e & 15;
+          sc[e >> 4][i] = sees(sight, a.sinks, key0 + (e >> 4) * 32 + 8 * (i >> 2) + 4 * half + (i & 3)) ? sc[e >> 4][i] : kNegInf;
+          top_of(sc, e);
+        }
+        top = all_tops();
+      }
+      top *= a.scale_log2;
+      // The maximum moves only when it grows by more than 2^8: weights then reach
+      // 2^8 at most, and most tiles leave the outputs unscaled.
+      const float m_new = top > m_run + 8.0f ? top : m_run;
+      if (__any(m_new != m_run)) {
+        const float scale = m_new == kNegInf ? 1.0f : exp2_fast(m_run - m_new);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sums[i] *= scale;
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) acc[b] *= scale;
+        m_run = m_new;
+        hold();
+      }
+      m_use = m_run == kNegInf ? 0.0f : m_run;
+    };
+    auto weigh = [&](const f32x16 (&sc)[kKeyBlocks], int e) KVC_INLINE {
+      const int kb = e >> 4, i = e & 15;
+      const float p0 = exp2_fast(fmaf(sc[kb][i], a.scale_log2, -m_use)), p1 = exp2_fast(fmaf(sc[kb][i + 1], a.scale_log2, -m_use));
+      sums[i >> 1 & 3] += p0 + p1;
+      u32x4 w = __builtin_bit_cast(u32x4, pf[kb][i >> 3]);
+      w[i >> 1 & 3] = E::pack(p0, p1);
+      pf[kb][i >> 3] = __builtin_bit_cast(vec_t, w);
+    };
+
+    if constexpr (L::kGroups == 1) {
+      // One group: a tile's weights are formed beside the scores' products of the
+      // next one.
+      load(a.k, place_of(t_begin), kst);
+      load(a.v, place_of(t_begin), vst);
+      uint32_t there = place_of(t_begin).bytes != 0;  // whether the tiles from t on are in the pool, t lowest
+      store_k(0);
+      store_v(0);
+      Place ahead = place_of(t_begin + 1);
+      there |= static_cast<uint32_t>(ahead.bytes != 0) << 1;
+      load(a.k, ahead, kst);
+      load(a.v, ahead, vst);
+      store_k(1);
+      ahead = place_of(t_begin + 2);  // of tile t + 2
+      there |= static_cast<uint32_t>(ahead.bytes != 0) << 2;
+      load(a.k, ahead, kst);
+      ready(t_begin + 3);
+      __syncthreads();
+      f32x16 sc[2][kKeyBlocks];
+#pragma unroll
+      for (int i = 0; i < kScores; ++i) {
+        const int kb = i % kKeyBlocks, st = i / kKeyBlocks;
+        sc[0][kb] = E::mfma32(k_operand(0, i), qf[st], st ? sc[0][kb] : kZero);
+      }
+      tops[0] = tops[1] = tops[2] = tops[3] = kNegInf;
+#pragma unroll
+      for (int e = 0; e < kLane; ++e) top_of(sc[0], e);
+      float top = all_tops();
+      __syncthreads();
+      auto turn = [&](auto parity, int t) KVC_INLINE {
+        constexpr int own = decltype(parity)::value, other = 1 - own;  // of tile t and t + 1: buffers, scores
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) ring[i] = k_operand(other, i);
+        // No key of a page outside the pool is seen: its tile lies behind every row.
+        key0 = there & 1 ? range.tile(t) << L::kShift : 1 << 30;
+        hold();
+        prepare(sc[own], top);
+        Search search;
+        tops[0] = tops[1] = tops[2] = tops[3] = kNegInf;
+        products(std::true_type{}, sc[other], other, own, [&](int i) KVC_INLINE {
+#pragma unroll
+          for (int e = 0; e < kLane; e += 2)
+            if (i == e / 2 * kScores / (kLane / 2)) weigh(sc[own], e);
+          if (i == 1) store_k(own);    // tile t + 2; tile t's K was last read a barrier ago
+          if (i == 3) store_v(other);  // tile t + 1
+          if (i >= 4 && i < 8) seek(search, t + 3, i - 4);
+          if (i == 8) load(a.v, ahead, vst);
+          if (i == 9) load(a.k, search.at, kst);
+          constexpr int kFrom = kScores + 2, kTo = kScores + kValues;  // the scores are there
+#pragma unroll
+          for (int e = 0; e < kLane; ++e)
+            if (i == kFrom + e / 2 * 2 * (kTo - kFrom) / kLane) top_of(sc[other], e);
+          if (i == kTo - 1) top = all_tops();
+        });
+        ahead = search.at;
+        there = there >> 1 | static_cast<uint32_t>(search.at.bytes != 0) << 2;
+        ready(t + 4);
+        __syncthreads();
+      };
+      for (int t = t_begin; t < t_end; t += 2) {
+        turn(std::integral_constant<int, 0>{}, t);
+        turn(std::integral_constant<int, 1>{}, t + 1);  // no key of a tile behind the last one is seen
+      }
+    } else {
+      f32x16 sc[kKeyBlocks];
+      // The first tile of K, a tile of zeros as V before it, and what the second group
+      // stores ahead; the next ones wait in registers.
+      int now = 0, next = 1, before = 2;  // buffers of tiles t, t + 1 and t - 1
+      Place old = place_of(t_begin);
+      uint32_t there = old.bytes != 0;  // whether the last tiles that were asked for are in the pool, the latest lowest
+      load(a.k, old, kst);
+      store_k(now);
+#pragma unroll
+      for (int i = 0; i < L::kLoads; ++i) vst[i] = u32x4{0, 0, 0, 0};
+      store_v(before);
+      Place ahead = place_of(t_begin + 1);
+      load(a.k, ahead, kst);
+      load(a.v, old, vst);
+      there = there << 1 | (ahead.bytes != 0);
+      old = ahead;
+      if (group) {
+        store_k(next);
+        store_v(now);
+        ahead = place_of(t_begin + 2);
+        load(a.k, ahead, kst);
+        load(a.v, old, vst);
+        there = there << 1 | (ahead.bytes != 0);
+        old = ahead;
+      }
+      ready(t_begin + 2 + group);
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) ring[i] = k_operand(now, i);
+      if (group) __syncthreads();
+      for (int t = t_begin; t < t_end; ++t) {
+        // Products, beside them the tiles that wait in registers go to LDS, the ones
+        // behind those are asked for, and the scores' maximum is taken.
+        Search search;
+        float top;
+        tops[0] = tops[1] = tops[2] = tops[3] = kNegInf;
+        __builtin_amdgcn_s_setprio(1);
+        products(std::true_type{}, sc, now, before, [&](int i) KVC_INLINE {
+          if (i == 1) store_k(group ? before : next);
+          if (i == 2) store_v(group ? next : now);
+          if (i >= 3 && i < 7) seek(search, t + 2 + group, i - 3);
+          if (i == 7) load(a.v, old, vst);
+          if (i == 8) load(a.k, search.at, kst);
+          constexpr int kFrom = kScores + 2, kTo = kScores + kValues;  // the scores are there
+#pragma unroll
+          for (int e = 0; e < kLane; ++e)
+            if (i == kFrom + e / 2 * 2 * (kTo - kFrom) / kLane) top_of(sc, e);
+          if (i == kTo - 1) top = all_tops();
+        });
+        __builtin_amdgcn_s_setprio(0);
+        there = there << 1 | (search.at.bytes != 0);
+        old = search.at;
+        // No key of a page outside the pool is seen: its tile lies behind every row.
+        key0 = there >> (2 + group) & 1 ? range.tile(t) << L::kShift : 1 << 30;
+        __syncthreads();
+        __builtin_amdgcn_sched_barrier(0);
+        // Softmax.
+        prepare(sc, top);
+#pragma unroll
+        for (int e = 0; e < kLane; e += 2) weigh(sc, e);
+        ready(t + 3 + group);
+        // The next products' first operands: they have been there for a phase.
+        const int free = before;
+        before = now;
+        now = next;
+        next = free;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) ring[i] = k_operand(now, i);
+        __builtin_amdgcn_sched_barrier(0);
+        // Nothing was stored since the last barrier: no wait for LDS before this one.
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) ring[i] = v_operand(before, i);
+      products(std::false_type{}, sc, now, before, [](int) {});
+      if (!group) __syncthreads();
     }
-  } else {
-  f32x16 sc[kKeyBlocks];
-  // The first tile of K, a tile of zeros as V before it, and what the second group
-  // stores ahead; the next ones wait in registers.
-  int now = 0, next = 1, before = 2;  // buffers of tiles t, t + 1 and t - 1
-  Place old = place_of(t_begin);
-  uint32_t there = old.bytes != 0;  // whether the last tiles that were asked for are in the pool, the latest lowest
-  load(a.k, old, kst);
-  store_k(now);
+    l_run = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    bool wild = false;
 #pragma unroll
-  for (int i = 0; i < L::kLoads; ++i) vst[i] = u32x4{0, 0, 0, 0};
-  store_v(before);
-  Place ahead = place_of(t_begin + 1);
-  load(a.k, ahead, kst);
-  load(a.v, old, vst);
-  there = there << 1 | (ahead.bytes != 0);
-  old = ahead;
-  if (group) {
-    store_k(next);
-    store_v(now);
-    ahead = place_of(t_begin + 2);
-    load(a.k, ahead, kst);
-    load(a.v, old, vst);
-    there = there << 1 | (ahead.bytes != 0);
-    old = ahead;
-  }
-  ready(t_begin + 2 + group);
-  __syncthreads();
+    for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
-  for (int i = 0; i < kAhead; ++i) ring[i] = k_operand(now, i);
-  if (group) __syncthreads();
-  for (int t = t_begin; t < t_end; ++t) {
-    // Products, beside them the tiles that wait in registers go to LDS, the ones
-    // behind those are asked for, and the scores' maximum is taken.
-    Search search;
-    float top;
-    tops[0] = tops[1] = tops[2] = tops[3] = kNegInf;
-    __builtin_amdgcn_s_setprio(1);
-    products(std::true_type{}, sc, now, before, [&](int i) KVC_INLINE {
-      if (i == 1) store_k(group ? before : next);
-      if (i == 2) store_v(group ? next : now);
-      if (i >= 3 && i < 7) seek(search, t + 2 + group, i - 3);
-      if (i == 7) load(a.v, old, vst);
-      if (i == 8) load(a.k, search.at, kst);
-      constexpr int kFrom = kScores + 2, kTo = kScores + kValues;  // the scores are there
-#pragma unroll
-      for (int e = 0; e < kLane; ++e)
-        if (i == kFrom + e / 2 * 2 * (kTo - kFrom) / kLane) top_of(sc, e);
-      if (i == kTo - 1) top = all_tops();
-    });
-    __builtin_amdgcn_s_setprio(0);
-    there = there << 1 | (search.at.bytes != 0);
-    old = search.at;
-    // No key of a page outside the pool is seen: its tile lies behind every row.
-    key0 = there >> (2 + group) & 1 ? range.tile(t) << L::kShift : 1 << 30;
-    __syncthreads();
-    __builtin_amdgcn_sched_barrier(0);
-    // Softmax.
-    prepare(sc, top);
-#pragma unroll
-    for (int e = 0; e < kLane; e += 2) weigh(sc, e);
-    ready(t + 3 + group);
-    // The next products' first operands: they have been there for a phase.
-    const int free = before;
-    before = now;
-    now = next;
-    next = free;
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) ring[i] = k_operand(now, i);
-    __builtin_amdgcn_sched_barrier(0);
-    // Nothing was stored since the last barrier: no wait for LDS before this one.
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-  }
-#pragma unroll
-  for (int i = 0; i < kAhead; ++i) ring[i] = v_operand(before, i);
-  products(std::false_type{}, sc, now, before, [](int) {});
-  if (!group) __syncthreads();
-  }
-  l_run = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-  bool wild = false;
-#pragma unroll
-  for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) wild |= !(fabsf(acc[b][i]) <= 3.4e38f);
-  return wild;
+      for (int i = 0; i < 16; ++i) wild |= !(fabsf(acc[b][i]) <= 3.4e38f);
+    return wild;
   };
   if (__syncthreads_or(go_over(std::false_type{}))) go_over(std::true_type{});
 
