@@ -49,6 +49,7 @@ AttendPlan make_plan(int kv_heads, int qpk, int head_dim, int n_seq, int64_t num
     const int64_t tiles = rows / many_rows(dim) + (most < n_seq ? most : n_seq);
     p.many.round = kCompute;  // one workgroup a compute unit
     p.many.grid = tiles * kv_heads + p.many.round;
+    p.many.most_tiles = static_cast<uint32_t>(tiles);
     const int64_t by_keys = pages * kBlockSize / 512;
     p.many.most_splits = static_cast<int>(by_keys < 1 ? 1 : (by_keys > p.many.round ? p.many.round : by_keys));
     if (p.many.most_splits > 1) many = static_cast<size_t>(p.many.round) * piece_floats(many_rows(dim), dim) * 4;

@@ -254,6 +254,7 @@ __device__ __forceinline__ void join_pieces(int count, int first, int rows, int 
 // launched, and a (row tile, head)'s keys are split at most `most_splits` times.
 struct ManyGrid {
   int round, most_splits;
+  uint32_t most_tiles;  // row tiles that the grid and the workspace are for
   int64_t grid;
 };
 

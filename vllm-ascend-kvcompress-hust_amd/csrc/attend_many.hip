@@ -73,17 +73,21 @@ struct ManyLayout {
 
 // Row tiles of a request that are this kernel's.
 template <int ROWS>
-__device__ __forceinline__ int tiles_of(const AttendArgs& a, const Request& s) {
+__device__ __forceinline__ uint32_t tiles_of(const AttendArgs& a, const Request& s) {
   const int64_t rows = static_cast<int64_t>(s.fresh) * a.qpk;
-  return rows > a.few_rows ? static_cast<int>((rows + ROWS - 1) / ROWS) : 0;
+  return rows > a.few_rows ? static_cast<uint32_t>((rows + ROWS - 1) / ROWS) : 0;
 }
 
-__device__ __forceinline__ int sum_up_to_lane(int x) {
+// Sums stop at `most` < 2^31, what the launch is for: starts that overlap name
+// more tokens than there are.
+__device__ __forceinline__ uint32_t add_up_to(uint32_t most, uint32_t x, uint32_t y) { return x + y < most ? x + y : most; }
+
+__device__ __forceinline__ uint32_t sum_up_to_lane(uint32_t most, uint32_t x) {
   const int lane = threadIdx.x & 63;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
-    const int up = __shfl_up(x, d);
-    if (lane >= d) x += up;
+    const uint32_t up = __shfl_up(x, d);
+    if (lane >= d) x = add_up_to(most, x, up);
   }
   return x;
 }
@@ -91,40 +95,42 @@ __device__ __forceinline__ int sum_up_to_lane(int x) {
 // Row tiles of all requests, counted by one wave: a lane sums its share of them.
 template <int ROWS>
 struct TileCount {
-  int share, sum;  // requests a lane, tiles up to the end of the lane's
-  Request last;    // the lane's last request
-  __device__ __forceinline__ TileCount(const AttendArgs& a) {
+  int share;           // requests a lane
+  uint32_t sum, most;  // tiles up to the end of the lane's
+  Request last;        // the lane's last request
+  __device__ __forceinline__ TileCount(const AttendArgs& a, const ManyGrid& grid) : most(grid.most_tiles) {
     const int lane = threadIdx.x & 63;
     share = (a.n_seq + 63) / 64;
     last = Request{0, 0, 0, 0};
-    int mine = 0;
+    uint32_t mine = 0;
     for (int i = 0; i < share; ++i) {
       const int r = lane * share + i;
       if (r >= a.n_seq) break;
       last = request_of(a, r);
-      mine += tiles_of<ROWS>(a, last);
+      mine = add_up_to(most, mine, tiles_of<ROWS>(a, last));
     }
-    sum = sum_up_to_lane(mine);
+    sum = sum_up_to_lane(most, mine);
   }
-  __device__ __forceinline__ int total() const { return __builtin_amdgcn_readlane(sum, 63); }
+  __device__ __forceinline__ int total() const { return static_cast<int>(__builtin_amdgcn_readlane(sum, 63)); }
   // The request of row tile `tile` < total(), its number, and the tile's in it.
   __device__ __forceinline__ Request find(const AttendArgs& a, int tile, int* request, int* local) const {
-    const int at = __builtin_ctzll(__ballot(sum > tile));  // the first lane whose share ends behind it
-    int before = at ? __builtin_amdgcn_readlane(sum, at > 0 ? at - 1 : 0) : 0;
+    const uint32_t place = static_cast<uint32_t>(tile);
+    const int at = __builtin_ctzll(__ballot(sum > place));  // the first lane whose share ends behind it
+    uint32_t before = at ? __builtin_amdgcn_readlane(sum, at > 0 ? at - 1 : 0) : 0;
     if (share == 1) {  // a lane holds what would be read again, which would be waited for
       *request = at;
-      *local = tile - before;
+      *local = static_cast<int>(place - before);
       return {__builtin_amdgcn_readlane(last.token0, at), __builtin_amdgcn_readlane(last.fresh, at),
               __builtin_amdgcn_readlane(last.len, at), __builtin_amdgcn_readlane(last.keys, at)};
     }
     for (int base = at * share;; base += 64) {
       const int r = base + static_cast<int>(threadIdx.x & 63);
-      const int up = sum_up_to_lane(r < a.n_seq && r < (at + 1) * share ? tiles_of<ROWS>(a, request_of(a, r)) : 0);
-      const uint64_t behind = __ballot(before + up > tile);
+      const uint32_t up = sum_up_to_lane(most, r < a.n_seq && r < (at + 1) * share ? tiles_of<ROWS>(a, request_of(a, r)) : 0);
+      const uint64_t behind = __ballot(before + up > place);
       if (behind || base + 64 >= (at + 1) * share) {
         const int in = behind ? __builtin_ctzll(behind) : 0;
         *request = base + in;
-        *local = tile - before - (in ? __builtin_amdgcn_readlane(up, in > 0 ? in - 1 : 0) : 0);
+        *local = static_cast<int>(place - before - (in ? __builtin_amdgcn_readlane(up, in > 0 ? in - 1 : 0) : 0));
         return uniform_request_of(a, *request);
       }
       before += __builtin_amdgcn_readlane(up, 63);
@@ -169,7 +175,7 @@ __global__ __launch_bounds__(ManyLayout<DP>::kThreads, ManyLayout<DP>::kGroups) 
   // split end last.
   const int head = blockIdx.x % a.kv_heads;
   const int order = blockIdx.x / a.kv_heads;
-  const TileCount<kRows> counted(a);
+  const TileCount<kRows> counted(a, grid);
   const ManyShares shares(a, grid, counted.total());
   const bool divided = order >= shares.whole;
   const int splits = divided ? shares.splits : 1;
@@ -612,7 +618,7 @@ __global__ __launch_bounds__(kJoinThreads) void attend_many_join_kernel(AttendAr
   typedef AttendElem<F16> E;
   constexpr int kRows = many_rows(DP);
   const int head = blockIdx.x % a.kv_heads, item = blockIdx.x / a.kv_heads;
-  const TileCount<kRows> counted(a);
+  const TileCount<kRows> counted(a, grid);
   const ManyShares shares(a, grid, counted.total());
   const int tile = shares.total - 1 - shares.whole - item;
   if (tile < 0) return;
