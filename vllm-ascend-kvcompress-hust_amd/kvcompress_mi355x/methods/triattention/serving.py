@@ -51,13 +51,13 @@ def _call(device: torch.device, name: str, *args: object) -> None:
             _native.call(name, dev.stream_handle(device), *args)
 
 
-def _vector(tensor: torch.Tensor, name: str, dtype: torch.dtype, like: torch.Tensor, length: int | None = None) -> int:
-    """A contiguous vector on ``like``'s device; returns its address."""
+def _vector(tensor: torch.Tensor, name: str, dtype: torch.dtype, like: torch.Tensor, where: int, length: int | None = None) -> int:
+    """A contiguous vector on ``like``'s device, whose number is ``where``; returns its address."""
     if (
         tensor.dtype is dtype
+        and tensor.get_device() == where
         and tensor.dim() == 1
         and tensor.is_contiguous()
-        and tensor.get_device() == like.get_device()
         and (length is None or tensor.numel() == length)
     ):
         return tensor.data_ptr()
@@ -116,20 +116,19 @@ def build_step_tables(
     ``max_query_len`` (the longest request's new tokens, if the host knows it)
     only sizes the launch."""
     dev.require_hip(computed_tokens, "computed_tokens")
-    like = computed_tokens
-    n = computed_tokens.numel()
-    computed = _vector(computed_tokens, "computed_tokens", torch.int32, like)
-    new = _vector(new_tokens, "new_tokens", torch.int32, like, n)
-    offsets = None if request_offsets is None else _vector(request_offsets, "request_offsets", torch.int64, like, n)
-    ids = _vector(block_ids, "block_ids", torch.int64, like)
-    id_offsets = _vector(block_offsets, "block_offsets", torch.int64, like, n + 1)
-    start = _vector(query_start_loc, "query_start_loc", torch.int32, like, n + 1)
-    lens = _vector(seq_lens, "seq_lens", torch.int32, like)
+    like, where, n = computed_tokens, computed_tokens.get_device(), computed_tokens.numel()
+    computed = _vector(computed_tokens, "computed_tokens", torch.int32, like, where)
+    new = _vector(new_tokens, "new_tokens", torch.int32, like, where, n)
+    offsets = None if request_offsets is None else _vector(request_offsets, "request_offsets", torch.int64, like, where, n)
+    ids = _vector(block_ids, "block_ids", torch.int64, like, where)
+    id_offsets = _vector(block_offsets, "block_offsets", torch.int64, like, where, n + 1)
+    start = _vector(query_start_loc, "query_start_loc", torch.int32, like, where, n + 1)
+    lens = _vector(seq_lens, "seq_lens", torch.int32, like, where)
     if seq_lens.numel() < n:
         raise ValueError("seq_lens must have an entry for every request")
     tokens = positions.numel()
-    places = _vector(positions, "positions", torch.int64, like)
-    slots = _vector(slot_mapping, "slot_mapping", torch.int64, like, tokens)
+    places = _vector(positions, "positions", torch.int64, like, where)
+    slots = _vector(slot_mapping, "slot_mapping", torch.int64, like, where, tokens)
     stride, blocks = _block_table(block_table, n, like)
     longest = tokens if max_query_len is None else int(max_query_len)
     if longest < 0:
@@ -207,7 +206,8 @@ def rotate_and_store(
     new tensor."""
     code, pages, page_stride, kv_heads, dim = _cache_pair(k_cache, v_cache)
     tokens = slot_mapping.numel()
-    slots = _vector(slot_mapping, "slot_mapping", torch.int64, k_cache)
+    where = k_cache.get_device()
+    slots = _vector(slot_mapping, "slot_mapping", torch.int64, k_cache, where)
     *q_place, heads = _heads(q, "q", tokens, k_cache)
     *k_place, k_heads = _heads(k, "k", tokens, k_cache)
     *v_place, v_heads = _heads(v, "v", tokens, k_cache)
@@ -221,7 +221,7 @@ def rotate_and_store(
     if heads and out_place[0] == q_place[0] and out_place != q_place:
         raise ValueError("q_out may be q itself, but not another view of it")
     freq = omega.numel()
-    turns = _vector(omega, "omega", torch.float32, k_cache)
+    turns = _vector(omega, "omega", torch.float32, k_cache, where)
     if not 0 < 2 * freq <= dim:
         raise ValueError(f"omega must hold one to head_dim/2 = {dim // 2} frequencies, got {freq}")
     if positions.get_device() != k_cache.get_device():
@@ -301,10 +301,11 @@ def attend_paged(
     if heads == 0 or heads % kv_heads:
         raise ValueError(f"query heads ({heads}) must be a positive multiple of the cache's KV heads ({kv_heads})")
     n = query_start_loc.numel() - 1
-    start = _vector(query_start_loc, "query_start_loc", torch.int32, k_cache)
+    where = k_cache.get_device()
+    start = _vector(query_start_loc, "query_start_loc", torch.int32, k_cache, where)
     if n < 0:
         raise ValueError("query_start_loc must have one entry more than there are requests")
-    lens = _vector(seq_lens, "seq_lens", torch.int32, k_cache)
+    lens = _vector(seq_lens, "seq_lens", torch.int32, k_cache, where)
     if seq_lens.numel() < n:
         raise ValueError("seq_lens must have a row for every request")
     stride, blocks = _block_table(block_table, n, k_cache)
