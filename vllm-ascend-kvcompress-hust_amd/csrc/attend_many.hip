@@ -644,8 +644,9 @@ int launch(hipStream_t stream, const AttendArgs& a, const ManyGrid& grid) {
   attend_many_kernel<F16, DP><<<static_cast<unsigned>(grid.grid), ManyLayout<DP>::kThreads, 0, stream>>>(a, grid);
   if (int rc = launch_status("kvc_attend_paged")) return rc;
   // Split items number half a round at most: each has two splits or more.
+  const int64_t items = grid.grid - grid.round, split = items < grid.round / 2 ? items : grid.round / 2;
   if (grid.most_splits > 1)
-    attend_many_join_kernel<F16, DP><<<dim3(grid.round / 2, kRows / kJoinRows), kJoinThreads, 0, stream>>>(a, grid);
+    attend_many_join_kernel<F16, DP><<<dim3(static_cast<unsigned>(split), kRows / kJoinRows), kJoinThreads, 0, stream>>>(a, grid);
   return launch_status("kvc_attend_paged");
 }
 
