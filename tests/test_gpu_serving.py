@@ -300,7 +300,7 @@ def test_attend_short_requests_apart_from_chunks(hip_device, heads, kv, dim, dty
                rows_most=max(new) * heads // kv)
 
 
-@pytest.mark.parametrize("dim, dtype", [(128, BF16), (128, FP16), (256, BF16), (96, BF16)])
+@pytest.mark.parametrize("dim, dtype", [(128, BF16), (128, FP16), (256, BF16), (96, BF16), (192, BF16), (64, FP16), (256, FP16)])
 @pytest.mark.parametrize("new, window, sinks", [(3, 0, 0), (4, 7, 2), (60, 0, 0), (60, 9, 1)])
 def test_hidden_values_reach_no_row_that_does_not_see_them(hip_device, dim, dtype, new, window, sinks) -> None:
     """Infinities and NaN in keys and values that some rows see and others do
@@ -341,6 +341,24 @@ def test_pages_outside_the_pool_are_not_seen(hip_device, new) -> None:
     got = _serving().attend_paged(q.to(hip_device), k.to(hip_device), v.to(hip_device), d(start), d(lens), table.to(hip_device))
     _check(got, q, (k, v), start, lens, table, BF16, scale=dim**-0.5, window=0, sinks=0, rows_most=new * 4)
     assert (got[start[1] :] == 0).all()
+
+
+@pytest.mark.parametrize("new", [1, 6, 70])
+@pytest.mark.parametrize("dim, dtype", [(64, FP16), (96, BF16), (192, BF16), (192, FP16), (256, BF16)])
+def test_pages_outside_the_pool_at_other_head_sizes(hip_device, dim, dtype, new) -> None:
+    """Holes between a request's pages, at its first and last ones, odd and even
+    numbers of key tiles, with a window over some."""
+    g = torch.Generator().manual_seed(dim + new)
+    lens, heads, kv = [1500, 1000, 500, 129], 8, 2
+    k, v, table = _paged(lens, kv, dim, dtype, g)
+    table[0, 2:5], table[0, 7], table[1, 0], table[2, 3] = -1, k.shape[0], -1, 1 << 30
+    start = [0, new, 2 * new, 3 * new, 4 * new]
+    q = torch.randn((4 * new, heads, dim), generator=g).to(dtype)
+    d = lambda x: torch.tensor(x, dtype=torch.int32, device=hip_device)  # noqa: E731
+    for window, sinks in ((0, 0), (300, 130)):
+        got = _serving().attend_paged(q.to(hip_device), k.to(hip_device), v.to(hip_device), d(start), d(lens), table.to(hip_device),
+                                      max_query_len=new, window=window, sinks=sinks)
+        _check(got, q, (k, v), start, lens, table, dtype, scale=dim**-0.5, window=window, sinks=sinks, rows_most=new * 4)
 
 
 @pytest.mark.parametrize("new", [1, 3, 50])
@@ -466,6 +484,22 @@ def test_attend_splits_what_whole_rounds_leave(hip_device, tokens, total, kv, he
     lens = [total - tokens + i + 1 for i in picked]
     _check(got[picked], q[picked], (k, v), list(range(len(picked) + 1)), lens, table.expand(len(picked), -1), BF16, scale=dim**-0.5,
            window=window, sinks=0, rows_most=tokens)
+
+
+@pytest.mark.parametrize("tokens, total, kv, heads, dim, dtype", [
+    (300, 5000, 2, 8, 64, BF16), (300, 5000, 2, 8, 96, FP16), (300, 5000, 2, 8, 192, BF16), (300, 5000, 2, 8, 256, BF16),
+    (700, 2500, 8, 40, 256, FP16), (900, 2500, 8, 40, 192, BF16),
+])
+def test_attend_splits_at_other_head_sizes(hip_device, tokens, total, kv, heads, dim, dtype) -> None:
+    g = torch.Generator().manual_seed(dim)
+    k, v, table = _paged([total], kv, dim, dtype, g)
+    q = torch.randn((tokens, heads, dim), generator=g).to(dtype)
+    d = lambda x: torch.tensor(x, dtype=torch.int32, device=hip_device)  # noqa: E731
+    got = _serving().attend_paged(q.to(hip_device), k.to(hip_device), v.to(hip_device), d([0, tokens]), d([total]), table.to(hip_device))
+    picked = sorted({0, 1, 25, 26, 31, 32, 63, 64, tokens // 2, tokens - 27, tokens - 1})
+    lens = [total - tokens + i + 1 for i in picked]
+    _check(got[picked], q[picked], (k, v), list(range(len(picked) + 1)), lens, table.expand(len(picked), -1), dtype, scale=dim**-0.5,
+           window=0, sinks=0, rows_most=tokens)
 
 
 @pytest.mark.parametrize("new", [1, 40])
