@@ -328,6 +328,30 @@ def test_hidden_values_reach_no_row_that_does_not_see_them(hip_device, dim, dtyp
     assert ((got.double() - want).abs()[fine] <= 4 * torch.finfo(dtype).eps * (want.abs()[fine] + 1)).all()
 
 
+@pytest.mark.parametrize("dim, dtype", [(64, BF16), (96, FP16), (128, BF16), (192, FP16), (256, BF16)])
+@pytest.mark.parametrize("window, sinks", [(0, 0), (6, 2)])
+def test_hidden_values_beside_drafts_of_many_heads(hip_device, dim, dtype, window, sinks) -> None:
+    """The same for three tokens of eight heads a KV head, by tokens that see a
+    key and those that do not."""
+    g = torch.Generator().manual_seed(dim)
+    lens, heads, kv, new = [300, 131, 64], 16, 2, 3
+    k, v, table = _paged(lens, kv, dim, dtype, g)
+    for r, n in enumerate(lens):
+        for key, what in ((n - 1, float("inf")), (n - 2, float("nan")), (n - 9, float("-inf"))):
+            v[int(table[r, key // 128]), key % 128, r % 2, 1 + key % 7] = what
+    start = [0, new, 2 * new, 3 * new]
+    q = torch.randn((3 * new, heads, dim), generator=g).to(dtype)
+    d = lambda x: torch.tensor(x, dtype=torch.int32, device=hip_device)  # noqa: E731
+    got = _serving().attend_paged(q.to(hip_device), k.to(hip_device), v.to(hip_device), d(start), d(lens), table.to(hip_device),
+                                  max_query_len=new, window=window, sinks=sinks).cpu()
+    want, _, _ = ref.attend(q, k, v, start, lens, table, scale=dim**-0.5, window=window, sinks=sinks)
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(torch.isinf(got), torch.isinf(want)) and torch.equal(got[torch.isinf(got)].double(), want[torch.isinf(want)])
+    fine = torch.isfinite(want)
+    assert fine.any() and not fine.all()
+    assert ((got.double() - want).abs()[fine] <= 4 * torch.finfo(dtype).eps * (want.abs()[fine] + 1)).all()
+
+
 @pytest.mark.parametrize("new", [1, 40])
 def test_pages_outside_the_pool_are_not_seen(hip_device, new) -> None:
     g = torch.Generator().manual_seed(new)
