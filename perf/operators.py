@@ -17,7 +17,6 @@ Where ``own`` is false an operator runs in its plain form, in float32.
 
 from __future__ import annotations
 
-import functools
 import math
 import sys
 from pathlib import Path
@@ -221,7 +220,6 @@ def prepare(case, seed):
     return {"attend": _prepare_attend, "rotate": _prepare_rotate, "tables": _prepare_tables}[case["kind"]](case, seed)
 
 
-@functools.cache  # a user's program imports once, not at every call
 def _serving():
     root = str(Path(__file__).resolve().parents[1] / "vllm-ascend-kvcompress-hust_amd")
     if root not in sys.path:
