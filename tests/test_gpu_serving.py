@@ -352,6 +352,65 @@ def test_hidden_values_beside_drafts_of_many_heads(hip_device, dim, dtype, windo
     assert ((got.double() - want).abs()[fine] <= 4 * torch.finfo(dtype).eps * (want.abs()[fine] + 1)).all()
 
 
+@pytest.mark.parametrize("dim, heads, kv, new", [
+    (64, 2, 2, 1), (128, 4, 1, 1), (64, 16, 2, 3), (256, 8, 1, 2), (64, 4, 2, 40), (128, 16, 2, 6), (256, 4, 2, 20),
+])
+def test_small_weights_of_many_keys_add_up(hip_device, dim, heads, kv, new) -> None:
+    """fp16: a key of a large weight in each of the first page's four slices, and
+    131068 of 2^-25 of it, whose values are 0 and 1: the many add up to 2^-10.  A
+    hint of one key leaves all pages to one workgroup.
+
+    Bounds.  Output: half a step, 2^-11 of it.  Scores are one product of 16-bit
+    numbers each, exact; their float32 product with scale * log2(e), 25, is off by
+    25 * 2^-24 twice, a weight by ln 2 times that and an exponential's last bits:
+    2^-18.  Sums of positive numbers: at most 131072 / 32 products one after
+    another, each 2^-24 of the sum, 2^-12; the sum of the weights likewise.
+    Weights: one word, half a step, 2^-11, and 2^-36 of the largest each."""
+    length = 131072
+    k = torch.zeros((length // 128, 128, kv, dim), dtype=FP16, device=hip_device)
+    v = torch.ones_like(k)
+    k[0, 5::32, :, 3], v[0, 5::32] = 17.390625, 0.0
+    q = torch.zeros((new, heads, dim), dtype=FP16, device=hip_device)
+    q[..., 3] = 1.0
+    d = lambda x: torch.tensor(x, dtype=torch.int32, device=hip_device)  # noqa: E731
+    table = torch.arange(length // 128, dtype=torch.int32, device=hip_device)[None]
+    got = _serving().attend_paged(q, k, v, d([0, new]), d([length]), table, scale=1.0, max_query_len=new,
+                                  max_seq_len=1).double().cpu()
+    small = torch.arange(length - new - 3, length - 3, dtype=torch.float64)[:, None, None] * torch.exp(torch.tensor(-17.390625, dtype=torch.float64))
+    want = small / (4 + small)
+    bound = want * (2 * 2.0**-11 + 2 * 2.0**-12 + 2.0**-18) + length * 2.0**-36
+    assert ((got - want).abs() <= bound).all(), (float(got.min()), float(got.max()), float(want.min()))
+
+
+@pytest.mark.parametrize("dim, heads, new", [(64, 16, 1), (128, 8, 4), (256, 16, 1)])
+def test_two_words_of_a_small_weight(hip_device, dim, heads, new) -> None:
+    """fp16, few rows: weights of 2^-10 of the largest keep 2^-22 of their own.
+    Two of them meet values of opposite sign, so their difference shows.
+
+    Bounds.  Output: 2^-11 of it.  Scores are exact; times scale * log2(e) they
+    are at most 11, off by 11 * 2^-24 in the factor, the product and the
+    difference to the maximum: ln 2 * 33 * 2^-24 < 2^-19 of a weight, which
+    covers the exponential's last bit too; words: 2^-22."""
+    g = torch.Generator().manual_seed(dim)
+    k = torch.zeros((1, 128, 1, dim), dtype=FP16)
+    v = torch.zeros_like(k)
+    k[0, 0, 0, 0], k[0, 1, 0, 1] = 6.5, 1.0
+    v[0, 1], v[0, 2] = 32768.0, -32768.0
+    q = torch.zeros((new, heads, dim), dtype=FP16)
+    q[..., 0] = (1 + torch.rand((new, heads), generator=g) / 8).half()
+    q[..., 1] = (2.0**-11 * (1 + torch.rand((new, heads), generator=g))).half()
+    length = new + 3
+    d = lambda x: torch.tensor(x, dtype=torch.int32, device=hip_device)  # noqa: E731
+    got = _serving().attend_paged(q.to(hip_device), k.to(hip_device), v.to(hip_device), d([0, new]), d([length]), d([[0]]), scale=1.0,
+                                  max_query_len=new).double().cpu()
+    seen = torch.arange(length - new + 1, length + 1, dtype=torch.float64)[:, None]
+    first, second = (q[..., 0].double() * 6.5).exp(), q[..., 1].double().exp()
+    total = first + second + seen - 2
+    want = (32768 * (second - 1) / total)[..., None]
+    spread = (32768 * (second + 1) / total)[..., None]
+    assert ((got - want).abs() <= 2.0**-11 * want + spread * (2.0**-19 + 2.0**-22)).all()
+
+
 @pytest.mark.parametrize("new", [1, 40])
 def test_pages_outside_the_pool_are_not_seen(hip_device, new) -> None:
     g = torch.Generator().manual_seed(new)

@@ -283,7 +283,7 @@ __global__ __launch_bounds__(kFewThreads, few_residents(DP)) void attend_few_ker
           for (int j = 0; j < 8; ++j) top = fmaxf(top, x[j]);
           top = fmaxf(top, __shfl_xor(top, 16));
           top = max_across_halves(top);
-          const float m_new = fmaxf(m_run[n], top);
+          const float m_new = fmaxf(m_run[n], lowered<E::kRoom>(top));
           const float m_use = m_new == kNegInf ? 0.0f : m_new;
           const float scale = exp2_fast(m_run[n] - m_use);
           m_run[n] = m_new;
@@ -293,8 +293,9 @@ __global__ __launch_bounds__(kFewThreads, few_residents(DP)) void attend_few_ker
           for (int j = 0; j < 8; j += 2) {
             const float p0 = exp2_fast(x[j] - m_use), p1 = exp2_fast(x[j + 1] - m_use);
             sum += p0 + p1;
-            // Weights in two 16-bit words (2^-16 of them left, 2^-22 in fp16): the
-            // second product costs nothing beside the cache's bytes.
+            // Weights in two 16-bit words (2^-16 of them left; in fp16 2^-22, or
+            // 2^-40 of the row's largest): the second product costs nothing beside
+            // the cache's bytes.
             hw[j >> 1] = E::pack(p0, p1);
             lw[j >> 1] = E::pack(p0 - E::lo(hw[j >> 1]), p1 - E::hi(hw[j >> 1]));
           }

@@ -116,6 +116,10 @@ struct AttendElem : MfmaElem<F16> {
   typedef typename MfmaElem<F16>::vec vec;
   // Exponent bits: all set in infinities and NaN.
   static constexpr uint32_t kExponent = F16 ? 0x7c00u : 0x7f80u;
+  // A row's largest weight, as a power of two.  fp16 ends at 2^-24: with weights
+  // of at most 1 the ones below 2^-25 would be nothing, however many they are
+  // (131071 of 2^-25.1 make 2^-8).  bf16 has float32's exponents.
+  static constexpr int kRoom = F16 ? 15 : 0;
   __device__ __forceinline__ static f32x16 mfma32(vec a, vec b, f32x16 c) {
     if constexpr (F16)
       return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
@@ -189,6 +193,15 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t page_rsrc(const uint16_t* pool
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 constexpr float kNegInf = -__builtin_inff();
+
+// The exponent that a row's weights are taken from, whose largest score is `top`:
+// 2^(top - lowered) is 2^BY, and the sum of the weights grows with it.  Where
+// float32 has no fractions left a difference of BY may become 16, which fp16 does
+// not hold: such scores keep weights of at most 1.
+template <int BY>
+__device__ __forceinline__ float lowered(float top) {
+  return BY && fabsf(top) < 8388608.0f ? top - BY : top;
+}
 
 // Joins `count` pieces of ROWS rows (first, first + 1, .. below `rows`) of which
 // piece i is at piece(i): `floats` unnormalised outputs of DP dims a row, then

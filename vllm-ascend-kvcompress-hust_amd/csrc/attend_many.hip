@@ -381,6 +381,10 @@ __global__ __launch_bounds__(ManyLayout<DP>::kThreads, ManyLayout<DP>::kGroups) 
     auto top_of = [&](const f32x16 (&sc)[kKeyBlocks], int e) KVC_INLINE { tops[e & 3] = fmaxf(tops[e & 3], sc[e >> 4][e & 15]); };
     auto all_tops = [&]() KVC_INLINE { return max_across_halves(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]))); };
     constexpr int kLane = kKeyBlocks * 16;  // scores of a lane
+    // How far (as a power of two) weights may grow before the maximum moves.  fp16's
+    // room is shared with small weights: of the row's largest, half a step is kept
+    // down to 2^-25 and what is below 2^-36 is lost.
+    constexpr int kSlack = F16 ? 4 : 8;
     // The softmax of the scores in `sc`, whose maximum is `top`: masks and the
     // maximum, then the weights two by two, in `pf`.
     float m_use;
@@ -405,9 +409,10 @@ __global__ __launch_bounds__(ManyLayout<DP>::kThreads, ManyLayout<DP>::kGroups) 
         top = all_tops();
       }
       top *= a.scale_log2;
-      // The maximum moves only when it grows by more than 2^8: weights then reach
-      // 2^8 at most, and most tiles leave the outputs unscaled.
-      const float m_new = top > m_run + 8.0f ? top : m_run;
+      // The maximum moves only when it grows by more than kSlack: most tiles leave
+      // the outputs unscaled.
+      const float low = lowered<E::kRoom - kSlack>(top);
+      const float m_new = low > m_run + kSlack ? low : m_run;
       if (__any(m_new != m_run)) {
         const float scale = m_new == kNegInf ? 1.0f : exp2_fast(m_run - m_new);
 #pragma unroll
