@@ -365,7 +365,8 @@ def test_small_weights_of_many_keys_add_up(hip_device, dim, heads, kv, new) -> N
     25 * 2^-24 twice, a weight by ln 2 times that and an exponential's last bits:
     2^-18.  Sums of positive numbers: at most 131072 / 32 products one after
     another, each 2^-24 of the sum, 2^-12; the sum of the weights likewise.
-    Weights: one word, half a step, 2^-11, and 2^-36 of the largest each."""
+    Weights: one word, half a step, 2^-11, and 2^-34 of the largest each (fp16's
+    half step at its end, 2^-25, where the largest is held as 2^9)."""
     length = 131072
     k = torch.zeros((length // 128, 128, kv, dim), dtype=FP16, device=hip_device)
     v = torch.ones_like(k)
@@ -378,8 +379,27 @@ def test_small_weights_of_many_keys_add_up(hip_device, dim, heads, kv, new) -> N
                                   max_seq_len=1).double().cpu()
     small = torch.arange(length - new - 3, length - 3, dtype=torch.float64)[:, None, None] * torch.exp(torch.tensor(-17.390625, dtype=torch.float64))
     want = small / (4 + small)
-    bound = want * (2 * 2.0**-11 + 2 * 2.0**-12 + 2.0**-18) + length * 2.0**-36
+    bound = want * (2 * 2.0**-11 + 2 * 2.0**-12 + 2.0**-18) + length * 2.0**-34
     assert ((got - want).abs() <= bound).all(), (float(got.min()), float(got.max()), float(want.min()))
+
+
+@pytest.mark.parametrize("dim, new", [(64, 1), (128, 40), (192, 40), (256, 40)])
+def test_weights_of_huge_scores_stay_in_range(hip_device, dim, new) -> None:
+    """fp16: scores of 2^27 + 16 and, in later tiles, one float32 step more, 16.  A
+    row whose last keys have those gives their mean, as 2^-16 of 128 values of 1
+    beside 217 or more of 3 is less than half a step of 3."""
+    k = torch.zeros((4, 128, 1, dim), dtype=FP16)
+    v = torch.ones_like(k)
+    k[..., 0], k[..., 1] = 8192.0, 16.0
+    k[1:, ..., 1] = 32.0
+    v[1:] = 3.0
+    q = torch.zeros((new, 1, dim), dtype=FP16)
+    q[..., 0], q[..., 1] = 16384.0, 1.0
+    table = torch.tensor([[0, 1, 2, 3]], dtype=torch.int32, device=hip_device)
+    d = lambda x: torch.tensor(x, dtype=torch.int32, device=hip_device)  # noqa: E731
+    scale = 0.6931471824645996  # times float32's log2(e): exactly 1
+    got = _serving().attend_paged(q.to(hip_device), k.to(hip_device), v.to(hip_device), d([0, new]), d([384]), table, scale=scale)
+    assert (got == 3).all()
 
 
 @pytest.mark.parametrize("dim, heads, new", [(64, 16, 1), (128, 8, 4), (256, 16, 1)])

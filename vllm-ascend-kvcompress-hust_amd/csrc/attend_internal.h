@@ -195,9 +195,9 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 constexpr float kNegInf = -__builtin_inff();
 
 // The exponent that a row's weights are taken from, whose largest score is `top`:
-// 2^(top - lowered) is 2^BY, and the sum of the weights grows with it.  Where
-// float32 has no fractions left a difference of BY may become 16, which fp16 does
-// not hold: such scores keep weights of at most 1.
+// BY below it, so that its weight is 2^BY, in the sum of the weights as in the
+// outputs.  Where float32 has no fractions left that difference may become 16, and
+// fp16 ends below 2^16: there the largest weight is 1.
 template <int BY>
 __device__ __forceinline__ float lowered(float top) {
   return BY && fabsf(top) < 8388608.0f ? top - BY : top;

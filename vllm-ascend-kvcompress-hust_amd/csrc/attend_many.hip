@@ -381,10 +381,11 @@ __global__ __launch_bounds__(ManyLayout<DP>::kThreads, ManyLayout<DP>::kGroups) 
     auto top_of = [&](const f32x16 (&sc)[kKeyBlocks], int e) KVC_INLINE { tops[e & 3] = fmaxf(tops[e & 3], sc[e >> 4][e & 15]); };
     auto all_tops = [&]() KVC_INLINE { return max_across_halves(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]))); };
     constexpr int kLane = kKeyBlocks * 16;  // scores of a lane
-    // How far (as a power of two) weights may grow before the maximum moves.  fp16's
-    // room is shared with small weights: of the row's largest, half a step is kept
-    // down to 2^-25 and what is below 2^-36 is lost.
-    constexpr int kSlack = F16 ? 4 : 8;
+    // How far (as a power of two) weights may grow before the maximum moves.  fp16
+    // shares its room between that and small weights: of the row's largest, half a
+    // step is kept down to 2^-23 and what is below 2^-34 is lost.  With 4, 2^2 less,
+    // 2048 tokens over 16384 keys, head_dim 256, take 628 us, with 6 613, with 8 601.
+    constexpr int kSlack = F16 ? 6 : 8, kBelow = E::kRoom > kSlack ? E::kRoom - kSlack : 0;
     // The softmax of the scores in `sc`, whose maximum is `top`: masks and the
     // maximum, then the weights two by two, in `pf`.
     float m_use;
@@ -410,10 +411,11 @@ __global__ __launch_bounds__(ManyLayout<DP>::kThreads, ManyLayout<DP>::kGroups) 
       }
       top *= a.scale_log2;
       // The maximum moves only when it grows by more than kSlack: most tiles leave
-      // the outputs unscaled.
-      const float low = lowered<E::kRoom - kSlack>(top);
-      const float m_new = low > m_run + kSlack ? low : m_run;
-      if (__any(m_new != m_run)) {
+      // the outputs unscaled.  Their difference is exact where it decides: a sum with
+      // the maximum rounds to multiples of 16 where scores reach 2^27.
+      const bool moves = top - m_run > kSlack + kBelow;
+      if (__any(moves)) {
+        const float m_new = moves ? lowered<kBelow>(top) : m_run;
         const float scale = m_new == kNegInf ? 1.0f : exp2_fast(m_run - m_new);
 #pragma unroll
         for (int i = 0; i < 4; ++i) sums[i] *= scale;
