@@ -459,11 +459,11 @@ int kvc_rotate_and_store(kvc_stream_t stream, int dtype, int rope_style, int64_t
  * scale is positive.  out may not overlap q; its rows outside every request are
  * left as they were.  Scores, softmax and sums are float32; where max_query_len *
  * qpk is more than 32, weights may be rounded to the cache's type before the
- * product with V (half a step of it; in fp16 what is below 2^-23 of the row's
- * largest to 2^-34 of that), else they keep twice its bits (2^-16 of them in bf16;
- * in fp16 2^-22, or 2^-40 of the row's largest).  Results are
- * the same on every run with the same arguments.  page_stride below 2^31 elements,
- * max_blocks below 2^23, kv_heads * max_blocks at most 2^30.
+ * product with V and their sum (half a step of a weight; in fp16 what is below
+ * 2^-23 of the row's largest to 2^-34 of that), else they keep twice its bits
+ * (2^-16 of a weight in bf16; in fp16 2^-22, or 2^-40 of the row's largest).
+ * Results are the same on every run with the same arguments.  page_stride below
+ * 2^31 elements, max_blocks below 2^23, kv_heads * max_blocks at most 2^30.
  * workspace: kvc_attend_workspace_bytes of the same sizes (0 for sizes that are
  * refused), any contents; calls that overlap in time need one each.
  * No counterpart in the reference (its host's attention backend reads the cache). */

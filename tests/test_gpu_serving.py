@@ -431,6 +431,39 @@ def test_two_words_of_a_small_weight(hip_device, dim, heads, new) -> None:
     assert ((got - want).abs() <= 2.0**-11 * want + spread * (2.0**-19 + 2.0**-22)).all()
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("dim, heads, kv, new", [(64, 8, 2, 40), (96, 4, 2, 40), (128, 40, 8, 30), (192, 4, 1, 50), (256, 8, 2, 70)])
+def test_weights_of_chunks_add_up_to_one(hip_device, dim, heads, kv, new, dtype) -> None:
+    """Values of c and one step above it, in another share in each dim: outputs are
+    the mean, rounded, whatever step the weights lie off.  All keys but the first
+    have a weight of (1 + 0.98 half steps) / 2, which rounds down, or (for every
+    other head) of (1 + 3.02 half steps) / 2, which rounds up.
+
+    Bounds.  Output: half a step of it.  Weights: half a step, of the distance of
+    two values, which is one step of c; the first key's in proportion.  Sums of
+    positive numbers in float32: 600 / 16 products and as many additions, each
+    2^-24 of the sum: 2^-18."""
+    length, step = 600, torch.finfo(dtype).eps
+    k, v, table = _paged([length], kv, dim, dtype, torch.Generator().manual_seed(dim), hidden=0.0)
+    slots = (table[0, : -(-length // 128), None].long() * 128 + torch.arange(128)).reshape(-1)[:length]
+    share = (torch.arange(length)[:, None] * dim % (length + 1)) < (torch.arange(dim) * length / dim)[None]
+    v.view(-1, kv, dim)[slots] = torch.where(share, 1 + step, 1.0).to(dtype)[:, None]
+    # q.k of 0 for the first key, -x for the others, by the first two dims.
+    k.zero_()
+    k.view(-1, kv, dim)[slots[1:], :, 0] = -1.0
+    k.view(-1, kv, dim)[slots[1:], :, 1] = -1.0
+    off = torch.where(torch.arange(heads) % 2 == 0, 0.98, 3.02).double()
+    x = -torch.log((1 + off * step / 2) / 2)
+    q = torch.zeros((new, heads, dim), dtype=dtype)
+    q[..., 0] = x.to(dtype)
+    q[..., 1] = (x - x.to(dtype).double()).to(dtype)
+    d = lambda y: torch.tensor(y, dtype=torch.int32, device=hip_device)  # noqa: E731
+    got = _serving().attend_paged(q.to(hip_device), k.to(hip_device), v.to(hip_device), d([0, new]), d([length]), table.to(hip_device),
+                                  scale=1.0)
+    want, spread, _ = ref.attend(q, k, v, [0, new], [length], table, scale=1.0)
+    assert ((got.double().cpu() - want).abs() <= want * (step / 2 + 2.0**-18) + step * step / 2).all()
+
+
 @pytest.mark.parametrize("new", [1, 40])
 def test_pages_outside_the_pool_are_not_seen(hip_device, new) -> None:
     g = torch.Generator().manual_seed(new)

@@ -126,6 +126,13 @@ struct AttendElem : MfmaElem<F16> {
     else
       return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
+  // sum + the two values of a word, in float32.
+  __device__ __forceinline__ static float add_pair(uint32_t w, float sum) {
+    if constexpr (F16)
+      return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), __builtin_bit_cast(f16x2, 0x3c003c00u), sum, false);
+    else
+      return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, 0x3f803f80u), sum, false);
+  }
 };
 
 // Four 16-bit values of one column: the 16 lanes of a group give the addresses

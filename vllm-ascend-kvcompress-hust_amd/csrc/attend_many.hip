@@ -22,9 +22,10 @@
 // scores (its other half in lane ^ 32), so the softmax needs one exchange, and
 // the packed weights are the right operand of O^T = V^T P^T as they lie, keys
 // numbered to match: slot (lane/32, j) of 16 keys is key 8*(j/4) + 4*(lane/32)
-// + j%4.  Weights are rounded to the cache's 16-bit type for that product (the
-// error of a sum of them is that of one rounding, as the output's own is); the
-// maxima, sums and outputs stay in float32.
+// + j%4.  Weights are rounded to the cache's 16-bit type for that product, and the
+// rounded ones are what is summed, so that a row's weights add up to one: what is
+// left is half a step of how far the values lie from their mean, where the output's
+// own rounding is half a step of it.  The maxima, sums and outputs are float32.
 
 #include <type_traits>
 #include <utility>
@@ -429,9 +430,9 @@ __global__ __launch_bounds__(ManyLayout<DP>::kThreads, ManyLayout<DP>::kGroups) 
     auto weigh = [&](const f32x16 (&sc)[kKeyBlocks], int e) KVC_INLINE {
       const int kb = e >> 4, i = e & 15;
       const float p0 = exp2_fast(fmaf(sc[kb][i], a.scale_log2, -m_use)), p1 = exp2_fast(fmaf(sc[kb][i + 1], a.scale_log2, -m_use));
-      sums[i >> 1 & 3] += p0 + p1;
       u32x4 w = __builtin_bit_cast(u32x4, pf[kb][i >> 3]);
       w[i >> 1 & 3] = E::pack(p0, p1);
+      sums[i >> 1 & 3] = E::add_pair(w[i >> 1 & 3], sums[i >> 1 & 3]);
       pf[kb][i >> 3] = __builtin_bit_cast(vec_t, w);
     };
 
