@@ -463,7 +463,8 @@ int kvc_rotate_and_store(kvc_stream_t stream, int dtype, int rope_style, int64_t
  * 2^-23 of the row's largest to 2^-34 of that), else they keep twice its bits
  * (2^-16 of a weight in bf16; in fp16 2^-22, or 2^-40 of the row's largest).
  * Results are the same on every run with the same arguments.  page_stride below
- * 2^31 elements, max_blocks below 2^23, kv_heads * max_blocks at most 2^30.
+ * 2^31 elements, max_blocks below 2^23, kv_heads * max_blocks at most 2^30,
+ * num_tokens and n_seq below 2^24, num_tokens * qpk below 2^31 - 256.
  * workspace: kvc_attend_workspace_bytes of the same sizes (0 for sizes that are
  * refused), any contents; calls that overlap in time need one each.
  * No counterpart in the reference (its host's attention backend reads the cache). */

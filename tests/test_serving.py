@@ -220,6 +220,21 @@ def test_attend_entry_refusals(change, message) -> None:
     assert re.search(message, lib.kvc_last_error().decode()), lib.kvc_last_error()
 
 
+@pytest.mark.parametrize("tokens, qpk", [(1 << 23, 256), ((1 << 24) - 1, 1024), (1 << 21, 1024), ((1 << 24) - 2, 128)])
+def test_rows_past_32_bits_are_refused(launches, tokens, qpk) -> None:
+    """Rows are numbered in 32 bits, the last tile's places behind them too."""
+    from kvcompress_mi355x import _native
+
+    lib = _native.load()
+    assert tokens * qpk >= (1 << 31) - 256
+    assert lib.kvc_attend_workspace_bytes(1, qpk, 8, 1, tokens, tokens, 512) == 0
+    assert _attend_c(lib, kv=1, qpk=qpk, dim=8, page=128 * 8, tokens=tokens, longest=tokens, qt=8 * qpk, qh=8, ot=8 * qpk, oh=8) == _native.EINVAL
+    assert "num_tokens * qpk" in lib.kvc_last_error().decode()
+    with pytest.raises(ValueError, match="below 2\\^31"):
+        _serving().attend_workspace_bytes(qpk, 1, 8, 1, tokens, tokens, 512)
+    assert lib.kvc_attend_workspace_bytes(1, 64, 8, 1, (1 << 24) - 1, (1 << 24) - 1, 512) > 0
+
+
 def test_entries_without_work_return_before_any_launch() -> None:
     from kvcompress_mi355x import _native
 

@@ -8,6 +8,9 @@ namespace kvc {
 namespace {
 
 constexpr int kCompute = 256;  // compute units of the device
+// Rows (tokens x query heads a KV head) of a call: the kernels number them, and the
+// places of a last tile behind them, in 32 bits.
+constexpr int64_t kMostRows = (1ll << 31) - 256;
 
 // How a call is launched; the workspace query and the call agree by sharing it.
 struct AttendPlan {
@@ -61,7 +64,8 @@ AttendPlan make_plan(int kv_heads, int qpk, int head_dim, int n_seq, int64_t num
 
 bool good_shape(int kv_heads, int qpk, int head_dim, int n_seq, int64_t num_tokens, int max_query_len, int max_seq_len) {
   return kv_heads > 0 && qpk > 0 && kv_heads <= 1024 && qpk <= 1024 && head_dim > 0 && head_dim % 8 == 0 && padded_dim(head_dim) &&
-         n_seq >= 0 && num_tokens >= 0 && num_tokens < (1 << 24) && n_seq < (1 << 24) && max_query_len >= 0 && max_seq_len >= 0;
+         n_seq >= 0 && num_tokens >= 0 && num_tokens < (1 << 24) && n_seq < (1 << 24) && max_query_len >= 0 && max_seq_len >= 0 &&
+         num_tokens * qpk < kMostRows;
 }
 
 }  // namespace
@@ -85,7 +89,7 @@ extern "C" int kvc_attend_paged(kvc_stream_t stream, int dtype, const void* q, i
   if (!good_shape(kv_heads, qpk, head_dim, n_seq, num_tokens, max_query_len, max_seq_len))
     return fail(KVC_EINVAL,
                 "kvc_attend_paged: bad sizes (head_dim %d must be a multiple of 8 up to 256; kv_heads %d, qpk %d at most 1024; "
-                "n_seq %d, num_tokens %lld below 2^24)",
+                "n_seq %d, num_tokens %lld below 2^24, num_tokens * qpk below 2^31 - 256)",
                 head_dim, kv_heads, qpk, n_seq, static_cast<long long>(num_tokens));
   if (num_pages < 0 || page_stride < static_cast<int64_t>(kBlockSize) * kv_heads * head_dim || page_stride % 8 ||
       page_stride >= (1ll << 31))

@@ -258,7 +258,10 @@ def attend_workspace_bytes(
         raise ValueError("query heads must be a multiple of the KV heads")
     size = _native.load().kvc_attend_workspace_bytes(kv_heads, heads // kv_heads, head_dim, n_seq, num_tokens, max_query_len, max_seq_len)
     if size == 0:
-        raise ValueError(f"unsupported attention shape (head_dim {head_dim} must be a multiple of 8 up to 256)")
+        raise ValueError(
+            f"unsupported attention shape (head_dim {head_dim} must be a multiple of 8 up to 256, tokens {num_tokens} below 2^24, "
+            f"tokens x query heads of a KV head below 2^31 - 256)"
+        )
     return int(size)
 
 
