@@ -410,8 +410,9 @@ int kvc_shift_lengths(kvc_stream_t stream, void* seq_lens, int elem_bytes, const
  * Tokens t >= query_start_loc[n_seq] (padding) get slot -1 and position 0.
  * Tokens past num_tokens are dropped: the request they belong to ends there and
  * the ones behind it bring none.  max_query_len sizes the launch only.  The
- * inputs may not overlap the outputs.  No counterpart in the reference, whose
- * host builds these (kvc_physical_slot_mapping replaces its hook). */
+ * inputs may not overlap the outputs.  n_seq below 2^24 - 1, num_tokens below 2^31.
+ * No counterpart in the reference, whose host builds these
+ * (kvc_physical_slot_mapping replaces its hook). */
 int kvc_step_tables(kvc_stream_t stream, int n_seq, const int32_t* computed_tokens, const int32_t* new_tokens,
                     const int64_t* request_offsets, const int64_t* block_ids, const int64_t* block_offsets,
                     int page_tokens, int max_query_len, int64_t num_tokens, int max_blocks, int64_t block_table_stride,

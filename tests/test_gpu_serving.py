@@ -156,6 +156,26 @@ def test_rotate_in_place_and_pass_through(hip_device) -> None:
     assert torch.equal(apart[0], q[0])  # position 0
 
 
+def test_rotate_more_tokens_than_one_dispatch_takes(hip_device) -> None:
+    """2^24 tokens of 256 threads: the values of two calls of about half of them."""
+    n, dim = (1 << 24) + 5, 8
+    g = torch.Generator(device=hip_device).manual_seed(8)
+    q, k, v = (torch.randn((n, 1, dim), generator=g, device=hip_device, dtype=BF16) for _ in range(3))
+    omega = torch.tensor([1.0, 0.5, 0.25, 0.125], device=hip_device)
+    positions = torch.randint(0, 1000, (2, n), generator=g, device=hip_device)
+    slots = torch.arange(n - 1, -1, -1, device=hip_device)
+    pages = -(-n // 128)
+    caches = [torch.zeros((pages, 128, 1, dim), dtype=BF16, device=hip_device) for _ in range(4)]
+    rotate = lambda part, *to: _serving().rotate_and_store(  # noqa: E731
+        q[part], k[part], v[part], positions[:, part], omega, slots[part], *to, sections=(3, 1))
+    whole = rotate(slice(0, n), *caches[:2])
+    half = (1 << 23) - 101
+    for part in (slice(0, half), slice(half, 2 * half), slice(2 * half, n)):
+        assert torch.equal(rotate(part, *caches[2:]), whole[part])
+    assert torch.equal(caches[0], caches[2]) and torch.equal(caches[1], caches[3])
+    assert torch.equal(caches[1].view(-1, 1, dim)[:n].flip(0), v)
+
+
 # --------------------------------------------------------------- attention --
 
 

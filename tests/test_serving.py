@@ -235,6 +235,17 @@ def test_rows_past_32_bits_are_refused(launches, tokens, qpk) -> None:
     assert lib.kvc_attend_workspace_bytes(1, 64, 8, 1, (1 << 24) - 1, (1 << 24) - 1, 512) > 0
 
 
+def test_launches_past_32_bits_of_work_items_are_refused() -> None:
+    from kvcompress_mi355x import _native
+
+    lib, fake, most = _native.load(), 4096, (1 << 24) - 1
+    # 2^19 row tiles x 1024 KV heads x 512 threads.
+    assert _attend_c(lib, kv=1024, qpk=8, dim=8, page=128 * 1024 * 8, tokens=most, longest=most, qt=8 * 8192, qh=8, ot=8 * 8192, oh=8) == _native.EINVAL
+    assert "too many rows" in lib.kvc_last_error().decode()
+    assert lib.kvc_step_tables(None, most, fake, fake, None, fake, fake, 128, 1, 5, 4, 8, fake, fake, fake, fake, fake) == _native.EINVAL
+    assert "bad sizes" in lib.kvc_last_error().decode()
+
+
 def test_entries_without_work_return_before_any_launch() -> None:
     from kvcompress_mi355x import _native
 

@@ -108,8 +108,9 @@ extern "C" int kvc_attend_paged(kvc_stream_t stream, int dtype, const void* q, i
   const AttendPlan plan = make_plan(kv_heads, qpk, head_dim, n_seq, num_tokens, max_query_len, max_seq_len);
   if (!workspace || workspace_bytes < plan.bytes)
     return fail(KVC_EINVAL, "kvc_attend_paged: workspace too small (%zu of %zu bytes)", workspace_bytes, plan.bytes);
-  if (plan.many.grid >= (1ll << 31))
-    return fail(KVC_EINVAL, "kvc_attend_paged: too many rows for one launch");
+  if (plan.many.grid * many_threads(padded_dim(head_dim)) > kMaxDispatchItems)
+    return fail(KVC_EINVAL, "kvc_attend_paged: too many rows for one launch (num_tokens * query heads / %d x %d threads, below 2^32)",
+                many_rows(padded_dim(head_dim)), many_threads(padded_dim(head_dim)));
 
   AttendArgs a = {};
   a.q = static_cast<const uint16_t*>(q);

@@ -288,6 +288,7 @@ constexpr int kFewTilesMost = 2;     // tiles of a request that the few-rows ker
 constexpr int kFewSequences = 1024;  // requests of one launch (their prefix sums sit in LDS)
 // Rows of one many-rows tile, 32 a wave.
 constexpr int many_rows(int dim) { return dim <= 192 ? 256 : 128; }
+constexpr int many_threads(int dim) { return many_rows(dim) * 2; }
 
 // Few-rows workgroups that a compute unit holds: as many as registers and LDS
 // allow, but for head_dim 64 and 96, where one more is slower (16 requests of

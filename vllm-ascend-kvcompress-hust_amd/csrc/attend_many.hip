@@ -64,7 +64,7 @@ struct ManyLayout {
   static constexpr int kTile = kKeys * kRow;
   static constexpr int kSlots = kRow / 8;
   static constexpr int kGroups = many_rows(DP) / 128;  // of four waves, 32 rows each
-  static constexpr int kThreads = 256 * kGroups;
+  static constexpr int kThreads = many_threads(DP);
   static constexpr int kBuffers = kGroups > 1 ? 3 : 2;  // of K and of V in LDS
   static constexpr int kStep = kThreads / kSlots;
   static constexpr int kLoads = kKeys / kStep;

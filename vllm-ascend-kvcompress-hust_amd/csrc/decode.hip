@@ -215,7 +215,8 @@ extern "C" int kvc_step_tables(kvc_stream_t stream, int n_seq, const int32_t* co
                                int page_tokens, int max_query_len, int64_t num_tokens, int max_blocks, int64_t block_table_stride,
                                int32_t* query_start_loc, int32_t* seq_lens, int64_t* positions, int64_t* slot_mapping,
                                int32_t* block_table) {
-  if (n_seq < 0 || n_seq >= (1 << 24) || num_tokens < 0 || num_tokens >= (1ll << 31) || max_query_len < 0)
+  // A workgroup a request and one for the padding, in one dispatch of less than 2^32 work-items.
+  if (n_seq < 0 || n_seq >= (1 << 24) - 1 || num_tokens < 0 || num_tokens >= (1ll << 31) || max_query_len < 0)
     return fail(KVC_EINVAL, "kvc_step_tables: bad sizes");
   if (page_tokens <= 0 || page_tokens % kBlockSize)
     return fail(KVC_EINVAL, "kvc_step_tables: page_tokens must be a positive multiple of %d", kBlockSize);

@@ -177,18 +177,36 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
   }
 }
 
+// Tokens of one dispatch, whose work-items are numbered in 32 bits.
+constexpr int64_t kRotaryTokens = 1 << 23;
+
 template <bool F16, bool IL>
-void launch(hipStream_t stream, const RotaryArgs& a, int64_t n, bool wide) {
+int launch(hipStream_t stream, RotaryArgs a, int64_t n, bool wide) {
   // Few tokens: the heads of one are spread over workgroups too.
   const int units = (a.heads + 2 * a.kv_heads) * (a.head_dim / (wide ? 8 : 1));
   const int64_t most = ceil_div(units, kRotaryThreads);
   int64_t shares = n >= 1024 ? 1 : ceil_div(1024, n);
   if (shares > most) shares = most;
-  const dim3 grid(static_cast<unsigned>(n), static_cast<unsigned>(shares));
-  if (wide)
-    rotary_kernel<F16, IL, 8><<<grid, kRotaryThreads, 0, stream>>>(a);
-  else
-    rotary_kernel<F16, IL, 1><<<grid, kRotaryThreads, 0, stream>>>(a);
+  while (n > 0) {
+    const int64_t now = n < kRotaryTokens ? n : kRotaryTokens;
+    const dim3 grid(static_cast<unsigned>(now), static_cast<unsigned>(shares));
+    if (wide)
+      rotary_kernel<F16, IL, 8><<<grid, kRotaryThreads, 0, stream>>>(a);
+    else
+      rotary_kernel<F16, IL, 1><<<grid, kRotaryThreads, 0, stream>>>(a);
+    if (int rc = launch_status("kvc_rotate_and_store")) return rc;
+    n -= now;
+    if (n == 0) break;
+    if (a.heads) {
+      a.q += now * a.q_token;
+      a.q_out += now * a.out_token;
+    }
+    a.k += now * a.k_token;
+    a.v += now * a.v_token;
+    a.positions += now;
+    a.slots += now;
+  }
+  return 0;
 }
 
 }  // namespace
@@ -265,9 +283,6 @@ extern "C" int kvc_rotate_and_store(kvc_stream_t stream, int dtype, int rope_sty
   const bool wide = bases % 16 == 0 && steps % 8 == 0 && a.freq % (il ? 4 : 8) == 0;
   const bool f16 = dtype == KVC_DTYPE_FP16;
   const hipStream_t st = as_stream(stream);
-  if (f16)
-    il ? launch<true, true>(st, a, num_tokens, wide) : launch<true, false>(st, a, num_tokens, wide);
-  else
-    il ? launch<false, true>(st, a, num_tokens, wide) : launch<false, false>(st, a, num_tokens, wide);
-  return launch_status("kvc_rotate_and_store");
+  if (f16) return il ? launch<true, true>(st, a, num_tokens, wide) : launch<true, false>(st, a, num_tokens, wide);
+  return il ? launch<false, true>(st, a, num_tokens, wide) : launch<false, false>(st, a, num_tokens, wide);
 }
