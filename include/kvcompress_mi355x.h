@@ -467,7 +467,8 @@ int kvc_rotate_and_store(kvc_stream_t stream, int dtype, int rope_style, int64_t
  * 2^31 elements, max_blocks below 2^23, kv_heads * max_blocks at most 2^30,
  * num_tokens and n_seq below 2^24, num_tokens * qpk below 2^31 - 256.
  * workspace: kvc_attend_workspace_bytes of the same sizes (0 for sizes that are
- * refused), any contents; calls that overlap in time need one each.
+ * refused) or, of the same heads and head_dim, of sizes none of which is smaller;
+ * any contents; calls that overlap in time need one each.
  * No counterpart in the reference (its host's attention backend reads the cache). */
 size_t kvc_attend_workspace_bytes(int kv_heads, int qpk, int head_dim, int n_seq, int64_t num_tokens,
                                   int max_query_len, int max_seq_len);

@@ -257,6 +257,19 @@ def test_entries_without_work_return_before_any_launch() -> None:
     assert lib.kvc_attend_workspace_bytes(0, 5, 128, 16, 16, 1, 16384) == 0
 
 
+@pytest.mark.parametrize("dim", [64, 128, 192, 256])
+@pytest.mark.parametrize("heads, kv", [(8, 1), (16, 8), (32, 1), (64, 8), (40, 1)])
+def test_workspace_of_the_largest_step_serves_smaller_ones(dim, heads, kv) -> None:
+    """No size needs less than a smaller one: a step of single tokens, of drafts, of
+    chunks, short requests and long ones, apart and in one launch."""
+    bytes_of = _serving().attend_workspace_bytes
+    sizes = [(n, n * new, new, longest) for n in (0, 1, 7, 64, 2000) for new in (0, 1, 2, 4, 5, 40, 700)
+             for longest in (0, 1, 128, 896, 1024, 5000, 65536)]
+    need = {s: bytes_of(heads, kv, dim, *s) for s in sizes}
+    for large, most in need.items():
+        assert all(least <= most for small, least in need.items() if all(a <= b for a, b in zip(small, large))), large
+
+
 @pytest.mark.parametrize("change, message", [
     ({"dtype": 2}, "dtype"), ({"style": 2}, "rope style"), ({"rotary": 130}, "rotary_dim"), ({"rotary": 63}, "rotary_dim"),
     ({"axes": 5}, "axes"), ({"axes": 0}, "axes"), ({"sections": (60, 5, 0, 0)}, "add up"), ({"sections": (70, -6, 0, 0)}, "section"),

@@ -17,7 +17,6 @@ struct AttendPlan {
   int row_tiles;    // 16-row tiles a request of the few-rows kernel has at most; 0: kernel not needed
   int workgroups;   // of the few-rows kernel
   ManyGrid many;    // of the many-rows kernel; no grid: kernel not needed
-  int sequences;    // requests of one few-rows launch
   size_t bytes;     // workspace
 };
 
@@ -35,13 +34,19 @@ AttendPlan make_plan(int kv_heads, int qpk, int head_dim, int n_seq, int64_t num
   //   63 of 4096, 8 KV heads       195 / 298 / 480, apart 185 / 263 / 482
   const bool together = most_rows > kFewRows * kFewTilesMost &&
                         static_cast<int64_t>(n_seq) * kv_heads * max_seq_len <= (1 << 19);
-  if (qpk <= kFewRows * kFewTilesMost && !together) {
-    p.row_tiles = most_rows <= kFewRows ? 1 : kFewTilesMost;
-    p.sequences = n_seq < kFewSequences ? n_seq : kFewSequences;
-    const int64_t bound = static_cast<int64_t>(p.sequences) * kv_heads * pages;
+  if (qpk <= kFewRows * kFewTilesMost) {
+    const int row_tiles = most_rows <= kFewRows ? 1 : kFewTilesMost;
+    const int64_t sequences = n_seq < kFewSequences ? n_seq : kFewSequences;
+    const int64_t bound = sequences * kv_heads * pages;
     const int64_t resident = kCompute * few_residents(dim);
-    p.workgroups = static_cast<int>(bound < resident ? bound : resident);
-    few = static_cast<size_t>(p.workgroups) * (16 + 8 * piece_floats(kFewRows * p.row_tiles, dim));
+    const int workgroups = static_cast<int>(bound < resident ? bound : resident);
+    // Asked for also where the many-rows kernel takes all: a workspace for the
+    // largest step then serves the smaller ones too.
+    few = static_cast<size_t>(workgroups) * (16 + 8 * piece_floats(kFewRows * row_tiles, dim));
+    if (!together) {
+      p.row_tiles = row_tiles;
+      p.workgroups = workgroups;
+    }
   }
   if (most_rows > kFewRows * p.row_tiles) {
     // Row tiles are at most as many as all rows fill, and a partly filled one more

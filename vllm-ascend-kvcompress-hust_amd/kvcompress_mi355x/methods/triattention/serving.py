@@ -253,7 +253,8 @@ def rotate_and_store(
 def attend_workspace_bytes(
     heads: int, kv_heads: int, head_dim: int, n_seq: int, num_tokens: int, max_query_len: int, max_seq_len: int
 ) -> int:
-    """Bytes of :func:`attend_paged`'s workspace for a step of these sizes."""
+    """Bytes of :func:`attend_paged`'s workspace for a step of these sizes, and for
+    any with none of the last four larger."""
     if kv_heads <= 0 or heads % kv_heads:
         raise ValueError("query heads must be a multiple of the KV heads")
     size = _native.load().kvc_attend_workspace_bytes(kv_heads, heads // kv_heads, head_dim, n_seq, num_tokens, max_query_len, max_seq_len)
