@@ -429,11 +429,12 @@ int kvc_step_tables(kvc_stream_t stream, int n_seq, const int32_t* computed_toke
  * runs in axis order, or (cycled) f%n_axes while f/n_axes < that axis's
  * section and axis 0 for the rest.  Element (t, h, d) of q is at
  * q[t*q_token_stride + h*q_head_stride + d], k and v likewise.  Turned queries
- * go to q_out (which may be q itself with the same strides, else may not overlap
- * it), turned keys and the values to row slot_mapping[t] of the cache
- * ([num_pages][128][kv_heads][head_dim]); slots outside [0, num_pages*128) store
- * nothing.  A slot may be named by one token only.  head_dim <= 1024,
- * rotary_dim <= 512.  No counterpart in the reference (its host's model does it). */
+ * go to q_out, which may be q itself with the same strides, else may not overlap
+ * it, and never k or v, nor its own rows each other; turned keys and the values go
+ * to row slot_mapping[t] of the cache ([num_pages][128][kv_heads][head_dim]); slots
+ * outside [0, num_pages*128) store nothing.  A slot may be named by one token only.
+ * head_dim <= 1024, rotary_dim <= 512.  No counterpart in the reference (its host's
+ * model does it). */
 int kvc_rotate_and_store(kvc_stream_t stream, int dtype, int rope_style, int64_t num_tokens, int heads, int kv_heads,
                          int head_dim, int rotary_dim, const void* q, int64_t q_token_stride, int64_t q_head_stride,
                          const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
@@ -457,8 +458,11 @@ int kvc_rotate_and_store(kvc_stream_t stream, int dtype, int rope_style, int64_t
  * strides in multiples of 8 elements, every pointer 16-byte aligned, head_dim a
  * multiple of 8 up to 256.  max_query_len must bound every request's new tokens
  * (rows of longer ones may be left out); max_seq_len sizes the launch only.
- * scale is positive.  out may not overlap q; its rows outside every request are
- * left as they were.  Scores, softmax and sums are float32; where max_query_len *
+ * scale is positive.  out may not overlap q, nor its own rows each other; its rows
+ * outside every request are left as they were.  (Of tensors whose address ranges
+ * meet it can only be told with the same token strides, and the same head strides
+ * or whole tokens' heads side by side, as in one projection: others are refused.)
+ * Scores, softmax and sums are float32; where max_query_len *
  * qpk is more than 32, weights may be rounded to the cache's type before the
  * product with V and their sum (half a step of a weight; in fp16 what is below
  * 2^-23 of the row's largest to 2^-34 of that), else they keep twice its bits

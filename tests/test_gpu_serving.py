@@ -541,6 +541,48 @@ def test_attend_strided_views_and_padded_pages(hip_device, new) -> None:
     assert torch.equal(got, plain) and (wide[..., dim:] == 5).all()
 
 
+@pytest.mark.parametrize("new", [1, 40])
+def test_outputs_beside_inputs_in_one_buffer(hip_device, new) -> None:
+    """Outputs between a projection's parts, heads taking turns, or tokens taking
+    turns are no overlap; the inputs themselves, shifted or widened, are."""
+    g = torch.Generator().manual_seed(new)
+    lens, heads, kv, dim, tokens = [500, 129], 8, 2, 64, 2 * new
+    k, v, table = (x.to(hip_device) for x in _paged(lens, kv, dim, BF16, g, hidden=0.0))
+    start = torch.tensor([0, new, 2 * new], dtype=torch.int32, device=hip_device)
+    seq = torch.tensor(lens, dtype=torch.int32, device=hip_device)
+    host = torch.randn((tokens, heads, dim), generator=g).to(BF16).to(hip_device)
+    attend = lambda q, out=None: _serving().attend_paged(q, k, v, start, seq, table, out=out)  # noqa: E731
+    plain = attend(host)
+    fused = torch.zeros((tokens, 3 * heads, dim), dtype=BF16, device=hip_device)
+    flat = torch.zeros((2 * heads, tokens, dim), dtype=BF16, device=hip_device)
+    turns = torch.zeros((tokens, 2, heads, dim), dtype=BF16, device=hip_device)
+    places = [(fused[:, heads : 2 * heads], fused[:, :heads]), (fused[:, :heads], fused[:, 2 * heads :]), (fused[:, 0 : 2 * heads : 2], fused[:, 1 : 2 * heads : 2]),
+              (flat[:heads].transpose(0, 1), flat[heads:].transpose(0, 1)), (flat[1::2].transpose(0, 1), flat[0::2].transpose(0, 1)),
+              (turns[:, 1], turns[:, 0])]
+    for q, out in places:
+        q.copy_(host)
+        out.fill_(7.0)
+        assert attend(q, out) is out and torch.equal(out, plain) and torch.equal(q, host)
+    q = fused[:, :heads].copy_(host)
+    for out in (q, fused[:, 1 : heads + 1], turns[:, 0, :1].expand(-1, heads, -1), turns[:1, 0].expand(tokens, -1, -1)):
+        with pytest.raises(ValueError, match="overlap"):
+            attend(q, out)
+    omega = torch.ones(dim // 2, device=hip_device)
+    positions, slots = torch.arange(tokens, device=hip_device), torch.arange(tokens, device=hip_device)
+    pages = [torch.zeros((2, 128, kv, dim), dtype=BF16, device=hip_device) for _ in range(2)]
+    kk, vv = (torch.randn((tokens, kv, dim), generator=g).to(BF16).to(hip_device) for _ in range(2))
+    rotate = lambda q, k, v, out=None: _serving().rotate_and_store(q, k, v, positions, omega, slots, *pages, q_out=out)  # noqa: E731
+    plain = rotate(host, kk, vv)
+    for q, out in places:
+        q.copy_(host)
+        assert torch.equal(rotate(q, kk, vv, out), plain) and torch.equal(q, host)
+        assert rotate(q, kk, vv, q) is q and torch.equal(q, plain)
+    q = fused[:, :heads].copy_(host)
+    for out in (fused[:, 1 : heads + 1], fused[:, heads : 2 * heads], turns[:, 0, :1].expand(-1, heads, -1)):
+        with pytest.raises(ValueError, match="overlap|another view"):
+            rotate(q, fused[:, heads : heads + kv], fused[:, 2 * heads - kv : 2 * heads], out)
+
+
 def test_attend_far_pages(hip_device) -> None:
     """Rows behind 2^32 elements of the pool, and slots behind 2^31 rows' bytes."""
     g = torch.Generator().manual_seed(5)

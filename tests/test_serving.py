@@ -246,6 +246,49 @@ def test_launches_past_32_bits_of_work_items_are_refused() -> None:
     assert "bad sizes" in lib.kvc_last_error().decode()
 
 
+# Two tokens of two heads of 128 elements, 2 bytes each: rows of 256 bytes, at 0, 256, 512 and 768.
+@pytest.mark.parametrize("change, message", [
+    ({}, "out overlaps q"),
+    ({"out": 4096 + 752}, "out overlaps q"),
+    ({"out": 4096 - 1008}, "out overlaps q"),
+    ({"qt": 512, "ot": 512, "out": 4096 + 256}, "out overlaps q"),  # the second head's rows are the first one's
+    ({"qt": 384, "ot": 384, "out": 4096 + 512 + 128}, "out overlaps q"),  # a token's rows end in the next one's
+    ({"ot": 512, "out": 4096 + 512}, "out overlaps q"),  # other strides in one range
+    ({"out": 8192, "oh": 0}, "rows of out"),
+    ({"out": 8192, "ot": 0}, "rows of out"),
+    ({"out": 8192, "oh": 120}, "rows of out"),
+    ({"out": 8192, "ot": 128, "oh": 128}, "rows of out"),  # the second token's first row is the first one's second
+    ({"out": 8192, "ot": 200, "oh": 128}, "rows of out"),
+])
+def test_attend_refuses_outputs_that_overlap(change, message) -> None:
+    from kvcompress_mi355x import _native
+
+    lib = _native.load()
+    assert _attend_c(lib, **{"tokens": 2, "longest": 2, **change}) == _native.EINVAL
+    assert message in lib.kvc_last_error().decode()
+
+
+@pytest.mark.parametrize("change, message", [
+    ({"out": 4096 + 16}, "without being q"),
+    ({"ot": 512}, "without being q"),
+    ({"out": (1 << 20) + 3 * 256}, "overlaps k or v"),
+    ({"out": (2 << 20) - 256}, "overlaps k or v"),
+    ({"out": 8 << 20, "oh": 0}, "rows of q_out"),
+    ({"out": 8 << 20, "ot": 64}, "rows of q_out"),
+])
+def test_rotary_refuses_outputs_that_overlap(change, message) -> None:
+    import ctypes
+
+    from kvcompress_mi355x import _native
+
+    lib, fake = _native.load(), 4096
+    a = {"out": fake, "ot": 256, "oh": 128, **change}
+    rc = lib.kvc_rotate_and_store(
+        None, 0, 0, 3, 2, 2, 128, 128, fake, 256, 128, 1 << 20, 256, 128, 2 << 20, 256, 128, fake, 0, 1, (ctypes.c_int * 1)(64), 0, fake, fake,
+        a["out"], a["ot"], a["oh"], fake, fake, 4, 128 * 2 * 128)
+    assert rc == _native.EINVAL and message in lib.kvc_last_error().decode()
+
+
 def test_entries_without_work_return_before_any_launch() -> None:
     from kvcompress_mi355x import _native
 

@@ -3,6 +3,7 @@
 #include <math.h>
 
 #include "attend_internal.h"
+#include "row_sets.h"
 
 namespace kvc {
 namespace {
@@ -116,6 +117,13 @@ extern "C" int kvc_attend_paged(kvc_stream_t stream, int dtype, const void* q, i
   if (plan.many.grid * many_threads(padded_dim(head_dim)) > kMaxDispatchItems)
     return fail(KVC_EINVAL, "kvc_attend_paged: too many rows for one launch (num_tokens * query heads / %d x %d threads, below 2^32)",
                 many_rows(padded_dim(head_dim)), many_threads(padded_dim(head_dim)));
+  // Tile numbers are 32-bit: requests x heads x pages of a few-rows launch stay below 2^30.
+  const int64_t each = static_cast<int64_t>(kv_heads) * (max_blocks > 0 ? max_blocks : 1);
+  if (plan.row_tiles && each > (1 << 30)) return fail(KVC_EINVAL, "kvc_attend_paged: kv_heads x max_blocks must be at most 2^30");
+  const RowSet read = row_set(q, q_token_stride, q_head_stride, num_tokens, kv_heads * qpk);
+  const RowSet written = row_set(out, out_token_stride, out_head_stride, num_tokens, kv_heads * qpk);
+  if (rows_share(written, 2 * head_dim)) return fail(KVC_EINVAL, "kvc_attend_paged: rows of out overlap each other");
+  if (rows_meet(written, read, 2 * head_dim)) return fail(KVC_EINVAL, "kvc_attend_paged: out overlaps q");
 
   AttendArgs a = {};
   a.q = static_cast<const uint16_t*>(q);
@@ -143,9 +151,6 @@ extern "C" int kvc_attend_paged(kvc_stream_t stream, int dtype, const void* q, i
   if (plan.row_tiles) {
     a.header = static_cast<int32_t*>(workspace);
     a.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + 16 * static_cast<size_t>(plan.workgroups));
-    // Tile numbers are 32-bit: requests x heads x pages of a launch stay below 2^30.
-    const int64_t each = static_cast<int64_t>(kv_heads) * (max_blocks > 0 ? max_blocks : 1);
-    if (each > (1 << 30)) return fail(KVC_EINVAL, "kvc_attend_paged: kv_heads x max_blocks must be at most 2^30");
     int64_t chunk = (1 << 30) / each;
     if (chunk > kFewSequences) chunk = kFewSequences;
     for (int64_t base = 0; base < n_seq; base += chunk) {

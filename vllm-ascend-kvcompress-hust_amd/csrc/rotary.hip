@@ -17,6 +17,7 @@
 
 #include "kvc_common.h"
 #include "mfma_common.h"
+#include "row_sets.h"
 
 namespace kvc {
 namespace {
@@ -248,6 +249,16 @@ extern "C" int kvc_rotate_and_store(kvc_stream_t stream, int dtype, int rope_sty
   if (num_tokens == 0) return 0;
   if ((heads > 0 && (!q || !q_out)) || !k || !v || !positions || !omega || !slot_mapping || (num_pages > 0 && (!k_cache || !v_cache)))
     return fail(KVC_EINVAL, "kvc_rotate_and_store: null pointer");
+  const RowSet turned = row_set(q_out, out_token_stride, out_head_stride, num_tokens, heads);
+  const RowSet queries = row_set(q, q_token_stride, q_head_stride, num_tokens, heads);
+  const int64_t row = 2 * head_dim;
+  if (rows_share(turned, row)) return fail(KVC_EINVAL, "kvc_rotate_and_store: rows of q_out overlap each other");
+  const bool in_place = turned.base == queries.base && turned.token == queries.token && turned.head == queries.head;
+  if (!in_place && rows_meet(turned, queries, row))
+    return fail(KVC_EINVAL, "kvc_rotate_and_store: q_out overlaps q without being q");
+  if (rows_meet(turned, row_set(k, k_token_stride, k_head_stride, num_tokens, kv_heads), row) ||
+      rows_meet(turned, row_set(v, v_token_stride, v_head_stride, num_tokens, kv_heads), row))
+    return fail(KVC_EINVAL, "kvc_rotate_and_store: q_out overlaps k or v");
   a.q = static_cast<const uint16_t*>(q);
   a.k = static_cast<const uint16_t*>(k);
   a.v = static_cast<const uint16_t*>(v);

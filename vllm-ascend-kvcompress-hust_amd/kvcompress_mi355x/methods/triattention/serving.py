@@ -202,8 +202,8 @@ def rotate_and_store(
     "half" pairs dims (f, F + f), "interleaved" (2f, 2f + 1).  Angles are formed
     in float64, rotations in float32, rounded once.  slot_mapping: int64
     [tokens], each slot at most once; tokens with a slot outside the cache (-1)
-    store nothing.  Returns the rotated queries: ``q_out`` (may be ``q``) or a
-    new tensor."""
+    store nothing.  Returns the rotated queries: ``q_out`` or a new tensor;
+    ``q_out`` may be ``q``, but overlap no other of the step's tensors."""
     code, pages, page_stride, kv_heads, dim = _cache_pair(k_cache, v_cache)
     tokens = slot_mapping.numel()
     where = k_cache.get_device()
@@ -296,7 +296,8 @@ def attend_paged(
     it.  ``max_query_len`` must bound every request's new tokens (default: all
     tokens); ``max_seq_len`` only sizes the launch (default: what the block
     table covers).  ``scale`` defaults to D ** -0.5.  ``out`` [tokens, heads, D]
-    may not overlap q; rows outside every request are not written.
+    may not overlap q or hold a row twice; rows outside every request are not
+    written.
     ``workspace``: uint8, at least :func:`attend_workspace_bytes`, for callers
     that keep one per stream; calls that overlap in time need one each."""
     code, pages, page_stride, kv_heads, dim = _cache_pair(k_cache, v_cache)
