@@ -409,8 +409,8 @@ int kvc_shift_lengths(kvc_stream_t stream, void* seq_lens, int elem_bytes, const
  *     where p is negative or has no page in the table (int64)
  * Tokens t >= query_start_loc[n_seq] (padding) get slot -1 and position 0.
  * Tokens past num_tokens are dropped: the request they belong to ends there and
- * the ones behind it bring none.  max_query_len sizes the launch only.  The
- * inputs may not overlap the outputs.  n_seq below 2^24 - 1, num_tokens below 2^31.
+ * the ones behind it bring none.  max_query_len sizes the launch only.  No
+ * output may overlap an input or another output.  n_seq below 2^24 - 1, num_tokens below 2^31.
  * No counterpart in the reference, whose host builds these
  * (kvc_physical_slot_mapping replaces its hook). */
 int kvc_step_tables(kvc_stream_t stream, int n_seq, const int32_t* computed_tokens, const int32_t* new_tokens,

@@ -81,6 +81,21 @@ def test_step_tables_without_requests(hip_device) -> None:
     assert start.tolist() == [0] and positions.tolist() == [0] * 6 and slots.tolist() == [-1] * 6
 
 
+def test_step_tables_beside_each_other_in_one_buffer(hip_device) -> None:
+    """Lengths in the gap behind a table's rows are no overlap; lengths written over
+    their own input are."""
+    d = lambda x, t=torch.int32: torch.tensor(x, dtype=t, device=hip_device)  # noqa: E731
+    wide = torch.full((3, 12), -7, dtype=torch.int32, device=hip_device)
+    args = (d([200, 5, 300]), d([1, 2, 1]), None, d([4, 9, 1, 2, 7, 8], torch.int64), d([0, 2, 3, 6], torch.int64), 128)
+    buffers = {"query_start_loc": wide[0, 4:8], "positions": torch.empty(4, dtype=torch.int64, device=hip_device),
+               "slot_mapping": torch.empty(4, dtype=torch.int64, device=hip_device), "block_table": wide[:, :4]}
+    _serving().build_step_tables(*args, seq_lens=wide[0, 8:11], **buffers)
+    assert wide.tolist() == [[4, 9, -1, -1, 0, 1, 3, 4, 201, 7, 301, -7], [1, -1, -1, -1] + [-7] * 8, [2, 7, 8, -1] + [-7] * 8]
+    for lens in (args[0], wide[0, 7:10], wide[1, :3]):
+        with pytest.raises(ValueError, match="overlap"):
+            _serving().build_step_tables(*args, seq_lens=lens, **buffers)
+
+
 # ------------------------------------------------------------------ rotary --
 
 ROTARY_CASES = [

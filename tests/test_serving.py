@@ -348,6 +348,32 @@ def test_step_tables_entry_refusals(change, message) -> None:
     assert rc == _native.EINVAL and message in lib.kvc_last_error().decode()
 
 
+# Tables of 3 requests and 5 tokens, 4096 bytes apart; 4 blocks of a row of 8.
+@pytest.mark.parametrize("change, message", [
+    ({"lens": 1}, "inputs and outputs"),  # lengths written over the computed tokens
+    ({"start": 2}, "inputs and outputs"),
+    ({"start": 2 - 3 / 1024}, "inputs and outputs"),  # its last entry is the first new token count
+    ({"slots": 3}, "inputs and outputs"),
+    ({"positions": 5 + 24 / 4096}, "inputs and outputs"),
+    ({"table": 1 - 64 / 4096}, "inputs and outputs"),  # its third row
+    ({"positions": 9}, "outputs overlap"),
+    ({"lens": 6 + 12 / 4096}, "outputs overlap"),
+    ({"table": 7 - 32 / 4096}, "outputs overlap"),  # its second row
+    ({"lens": 10 + 76 / 4096}, "outputs overlap"),
+    ({"lens": 10 + 8 / 4096}, "outputs overlap"),
+    ({"lens": 10 + 24 / 4096}, "outputs overlap"),  # two entries in the gap behind the first row (bytes 16 to 32), one in the second
+])
+def test_step_tables_refuse_tensors_that_overlap(change, message) -> None:
+    from kvcompress_mi355x import _native
+
+    lib = _native.load()
+    at = dict(computed=1, new=2, offsets=3, ids=4, id_offsets=5, start=6, lens=7, positions=8, slots=9, table=10)
+    a = {name: int(4096 * place) for name, place in {**at, **change}.items()}
+    rc = lib.kvc_step_tables(None, 3, a["computed"], a["new"], a["offsets"], a["ids"], a["id_offsets"], 128, 1, 5, 4, 8, a["start"], a["lens"],
+                             a["positions"], a["slots"], a["table"])
+    assert rc == _native.EINVAL and message in lib.kvc_last_error().decode()
+
+
 # ------------------------------------------------------- definitions by hand --
 
 

@@ -14,6 +14,7 @@
 // table itself, from the requests' lengths in one launch.
 
 #include "kvc_common.h"
+#include "row_sets.h"
 
 namespace kvc {
 namespace {
@@ -225,6 +226,24 @@ extern "C" int kvc_step_tables(kvc_stream_t stream, int n_seq, const int32_t* co
   if (!query_start_loc || (num_tokens > 0 && (!positions || !slot_mapping)) ||
       (n_seq > 0 && (!computed_tokens || !new_tokens || !block_offsets || !seq_lens || (max_blocks > 0 && !block_table))))
     return fail(KVC_EINVAL, "kvc_step_tables: null pointer");
+  // Workgroups read other requests' lengths while the tables are written.
+  const int64_t n = n_seq;
+  const Rows read[] = {vector_rows(computed_tokens, 4 * n), vector_rows(new_tokens, 4 * n), vector_rows(request_offsets, 8 * n),
+                       vector_rows(block_offsets, n ? 8 * (n + 1) : 0)};
+  const Rows written[] = {vector_rows(query_start_loc, 4 * (n + 1)), vector_rows(seq_lens, 4 * n), vector_rows(positions, 8 * num_tokens),
+                          vector_rows(slot_mapping, 8 * num_tokens)};
+  const Rows table = {static_cast<int64_t>(reinterpret_cast<uintptr_t>(block_table)), 4 * block_table_stride, max_blocks ? n : 0,
+                      4ll * max_blocks};
+  for (const Rows& x : read) {
+    bool meets = vector_meets(x, table);
+    for (const Rows& y : written) meets |= vector_meets(x, y);
+    if (meets) return fail(KVC_EINVAL, "kvc_step_tables: inputs and outputs overlap");
+  }
+  for (int i = 0; i < 4; ++i) {
+    bool meets = vector_meets(written[i], table);
+    for (int j = 0; j < i; ++j) meets |= vector_meets(written[i], written[j]);
+    if (meets) return fail(KVC_EINVAL, "kvc_step_tables: outputs overlap each other");
+  }
   // About four entries or tokens a thread, as far as the device has room for workgroups.
   const int64_t most = max_query_len > max_blocks ? max_query_len : max_blocks;
   int64_t shares = ceil_div(most, 4 * kDecodeThreads);

@@ -74,4 +74,22 @@ inline bool rows_meet(const RowSet& a, const RowSet& b, int64_t row) {
   return false;
 }
 
+// `count` rows of `row` bytes, `step` apart; a vector is one row.
+struct Rows {
+  int64_t base, step, count, row;
+};
+
+inline Rows vector_rows(const void* p, int64_t bytes) {
+  return {static_cast<int64_t>(reinterpret_cast<uintptr_t>(p)), 0, p && bytes > 0 ? 1 : 0, bytes};
+}
+
+// Whether a vector and a set of rows in address order share bytes.
+inline bool vector_meets(const Rows& v, const Rows& s) {
+  if (v.count < 1 || s.count < 1 || s.row < 1 || v.base + v.row <= s.base) return false;
+  const int64_t at = s.step > 0 && v.base > s.base ? (v.base - s.base) / s.step : 0;  // the last row that begins before it, or the first
+  const int64_t first = at < s.count ? at : s.count - 1;
+  if (v.base < s.base + first * s.step + s.row) return v.base + v.row > s.base + first * s.step;
+  return first + 1 < s.count && v.base + v.row > s.base + (first + 1) * s.step;
+}
+
 }  // namespace kvc

@@ -113,6 +113,7 @@ def build_step_tables(
     max_blocks] of 128-token pages with unit inner stride.  Entries behind a
     request's length and slots without a page are -1, padding tokens get slot
     -1 and position 0, rows of the tables behind request n stay as they were.
+    No written tensor may overlap another of the call's.
     ``max_query_len`` (the longest request's new tokens, if the host knows it)
     only sizes the launch."""
     dev.require_hip(computed_tokens, "computed_tokens")
