@@ -387,6 +387,61 @@ def test_hidden_values_beside_drafts_of_many_heads(hip_device, dim, dtype, windo
     assert ((got.double() - want).abs()[fine] <= 4 * torch.finfo(dtype).eps * (want.abs()[fine] + 1)).all()
 
 
+@pytest.mark.parametrize("dim, dtype", [(64, FP16), (128, BF16), (192, FP16), (256, BF16)])
+@pytest.mark.parametrize("new, window, sinks", [(1, 0, 0), (3, 1500, 4), (130, 0, 0), (130, 1500, 4), (300, 0, 0)])
+def test_hidden_values_in_pieces_that_are_joined(hip_device, dim, dtype, new, window, sinks) -> None:
+    """Infinities and NaN in some of the pieces that a request's keys are split into,
+    a piece of which holds no key for some rows: as many pieces as the launch is
+    for, by a hint of 20000 keys."""
+    g = torch.Generator().manual_seed(dim + new)
+    lens, heads, kv = [3000, 1700], 4, 2
+    k, v, table = _paged(lens, kv, dim, dtype, g, max_blocks=160)
+    for r, n in enumerate(lens):
+        first = n - new
+        for key, what in ((10, float("nan")), (first - 700, float("inf")), (first + new // 2, float("-inf")), (n - 1, float("nan")), (2, float("inf"))):
+            v[int(table[r, key // 128]), key % 128, r, 1 + key % 7] = what
+        v[int(table[r, (first - 300) // 128]), (first - 300) % 128, 1 - r, :] = float("inf")
+        key = first + new // 3
+        k[int(table[r, key // 128]), key % 128, 1 - r, 3] = float("nan")
+    start = [0, new, 2 * new]
+    q = (0.5 * torch.randn((2 * new, heads, dim), generator=g)).to(dtype)
+    d = lambda x: torch.tensor(x, dtype=torch.int32, device=hip_device)  # noqa: E731
+    got = _serving().attend_paged(q.to(hip_device), k.to(hip_device), v.to(hip_device), d(start), d(lens), table.to(hip_device),
+                                  max_query_len=new, max_seq_len=20000, window=window, sinks=sinks).cpu()
+    want, _, _ = ref.attend(q, k, v, start, lens, table, scale=dim**-0.5, window=window, sinks=sinks)
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(torch.isinf(got), torch.isinf(want)) and torch.equal(got[torch.isinf(got)].double(), want[torch.isinf(want)])
+    fine = torch.isfinite(want)
+    assert fine.any() and not fine.all()
+    assert ((got.double() - want).abs()[fine] <= 4 * torch.finfo(dtype).eps * (want.abs()[fine] + 1)).all()
+
+
+@pytest.mark.parametrize("dim, dtype", [(64, BF16), (128, BF16), (192, FP16), (256, BF16)])
+@pytest.mark.parametrize("lens, new", [([5000, 700, 3000], [1, 1, 1]), ([5000, 700, 3000], [4, 1, 3]), ([5000], [100]), ([4000, 2500], [90, 300]),
+                                       ([9000] * 16, [1, 200, 2, 1] * 4)])
+def test_workspace_of_split_calls(hip_device, dim, dtype, lens, new) -> None:
+    """Nothing behind the workspace is written and nothing it held before is read:
+    pieces of single tokens, drafts, chunks, and of both kinds after one another."""
+    serving = _serving()
+    g = torch.Generator(device=hip_device).manual_seed(dim)
+    heads, kv = 16, 4
+    pool = torch.randn((2, 300, 128, kv, dim), generator=g, device=hip_device).to(dtype)
+    table = torch.stack([torch.randperm(300, generator=g, device=hip_device)[:80] for _ in lens]).int()
+    q = torch.randn((sum(new), heads, dim), generator=g, device=hip_device).to(dtype)
+    d = lambda x: torch.tensor(x, dtype=torch.int32, device=hip_device)  # noqa: E731
+    start = d([0, *torch.tensor(new).cumsum(0).tolist()])
+    args = (q, pool[0], pool[1], start, d(lens), table)
+    sizes = {"max_query_len": max(new), "max_seq_len": max(lens)}
+    size = serving.attend_workspace_bytes(heads, kv, dim, len(lens), sum(new), *sizes.values())
+    outs = []
+    for fill in (0x00, 0xFF, 0x7F):
+        kept = torch.full((size + 4096,), fill, dtype=torch.uint8, device=hip_device)
+        outs.append(serving.attend_paged(*args, **sizes, workspace=kept[:size]))
+        assert (kept[size:] == fill).all()
+    outs.append(serving.attend_paged(*args, **sizes, workspace=kept[:size]))
+    assert all(torch.equal(out, outs[0]) for out in outs) and torch.isfinite(outs[0]).all()
+
+
 @pytest.mark.parametrize("dim, heads, kv, new", [
     (64, 2, 2, 1), (128, 4, 1, 1), (64, 16, 2, 3), (256, 8, 1, 2), (64, 4, 2, 40), (128, 16, 2, 6), (256, 4, 2, 20),
 ])
