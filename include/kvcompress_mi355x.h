@@ -432,7 +432,8 @@ int kvc_step_tables(kvc_stream_t stream, int n_seq, const int32_t* computed_toke
  * go to q_out, which may be q itself with the same strides, else may not overlap
  * it, and never k or v, nor its own rows each other; turned keys and the values go
  * to row slot_mapping[t] of the cache ([num_pages][128][kv_heads][head_dim]); slots
- * outside [0, num_pages*128) store nothing.  A slot may be named by one token only.
+ * outside [0, num_pages*128) store nothing.  A slot may be named by one token only,
+ * and the two caches may not be one.
  * head_dim <= 1024, rotary_dim <= 512.  No counterpart in the reference (its host's
  * model does it). */
 int kvc_rotate_and_store(kvc_stream_t stream, int dtype, int rope_style, int64_t num_tokens, int heads, int kv_heads,

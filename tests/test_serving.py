@@ -348,6 +348,18 @@ def test_step_tables_entry_refusals(change, message) -> None:
     assert rc == _native.EINVAL and message in lib.kvc_last_error().decode()
 
 
+def test_rotary_refuses_one_pool_for_keys_and_values() -> None:
+    import ctypes
+
+    from kvcompress_mi355x import _native
+
+    lib, fake = _native.load(), 4096
+    rc = lib.kvc_rotate_and_store(
+        None, 0, 0, 3, 2, 2, 128, 128, fake, 256, 128, 1 << 20, 256, 128, 2 << 20, 256, 128, fake, 0, 1, (ctypes.c_int * 1)(64), 0, fake, fake,
+        fake, 256, 128, 1 << 24, 1 << 24, 4, 128 * 2 * 128)
+    assert rc == _native.EINVAL and "one pool" in lib.kvc_last_error().decode()
+
+
 # Tables of 3 requests and 5 tokens, 4096 bytes apart; 4 blocks of a row of 8.
 @pytest.mark.parametrize("change, message", [
     ({"lens": 1}, "inputs and outputs"),  # lengths written over the computed tokens

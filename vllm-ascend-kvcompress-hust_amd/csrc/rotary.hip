@@ -259,6 +259,8 @@ extern "C" int kvc_rotate_and_store(kvc_stream_t stream, int dtype, int rope_sty
   if (rows_meet(turned, row_set(k, k_token_stride, k_head_stride, num_tokens, kv_heads), row) ||
       rows_meet(turned, row_set(v, v_token_stride, v_head_stride, num_tokens, kv_heads), row))
     return fail(KVC_EINVAL, "kvc_rotate_and_store: q_out overlaps k or v");
+  if (num_pages > 0 && k_cache == v_cache)
+    return fail(KVC_EINVAL, "kvc_rotate_and_store: k_cache and v_cache are one pool: keys and values would share its rows");
   a.q = static_cast<const uint16_t*>(q);
   a.k = static_cast<const uint16_t*>(k);
   a.v = static_cast<const uint16_t*>(v);
