@@ -754,6 +754,22 @@ def test_attend_splits_what_whole_rounds_leave(hip_device, tokens, total, kv, he
            window=window, sinks=0, rows_most=tokens)
 
 
+@pytest.mark.parametrize("heads, kv, dim, tokens, total", [(40, 8, 64, 10000, 10100), (24, 3, 64, 17000, 20000), (64, 8, 256, 3170, 6000)])
+def test_attend_splits_behind_many_rounds(hip_device, heads, kv, dim, tokens, total) -> None:
+    """Six rounds of (row tile, head) items and a few more, which are split as well."""
+    g = torch.Generator().manual_seed(tokens)
+    k, v, table = _paged([total], kv, dim, BF16, g)
+    q = torch.randn((tokens, heads, dim), generator=g).to(BF16)
+    d = lambda x: torch.tensor(x, dtype=torch.int32, device=hip_device)  # noqa: E731
+    got = _serving().attend_paged(q.to(hip_device), k.to(hip_device), v.to(hip_device), d([0, tokens]), d([total]), table.to(hip_device),
+                                  max_seq_len=total)
+    assert torch.isfinite(got).all()
+    picked = sorted({0, 1, 15, 16, 31, 32, 50, 51, 52, 300, tokens // 2, tokens - 27, tokens - 1})
+    lens = [total - tokens + i + 1 for i in picked]
+    _check(got[picked], q[picked], (k, v), list(range(len(picked) + 1)), lens, table.expand(len(picked), -1), BF16, scale=dim**-0.5,
+           window=0, sinks=0, rows_most=tokens)
+
+
 @pytest.mark.parametrize("tokens, total, kv, heads, dim, dtype", [
     (300, 5000, 2, 8, 64, BF16), (300, 5000, 2, 8, 96, FP16), (300, 5000, 2, 8, 192, BF16), (300, 5000, 2, 8, 256, BF16),
     (700, 2500, 8, 40, 256, FP16), (900, 2500, 8, 40, 192, BF16),

@@ -52,8 +52,9 @@ AttendPlan make_plan(int kv_heads, int qpk, int head_dim, int n_seq, int64_t num
   if (most_rows > kFewRows * p.row_tiles) {
     // Row tiles are at most as many as all rows fill, and a partly filled one more
     // for each request that has more rows than the few-rows kernel takes; one
-    // round more of workgroups is there for the items that are split, into no
-    // fewer than 512 keys.
+    // round more of workgroups is there for the items that are split, into one
+    // piece for every 512 keys of the longest request at most (a shorter one's
+    // pieces hold fewer keys, or none).
     const int64_t rows = num_tokens * qpk, most = rows / (kFewRows * p.row_tiles + 1);
     const int64_t tiles = rows / many_rows(dim) + (most < n_seq ? most : n_seq);
     p.many.round = kCompute;  // one workgroup a compute unit

@@ -141,14 +141,19 @@ struct TileCount {
 
 // How the (row tile, head) items are shared out: whole rounds of the device take
 // one item a workgroup; what is left over (or all, where there is no whole
-// round) is split along its keys into one more round.  From six rounds on, the
-// last, partly filled one is a small share and nothing is split.
-constexpr int kManyRounds = 6;
+// round) is split along its keys into one more round, however many rounds come
+// before it.  40 heads on 8, head_dim 128, split / left whole:
+//   1.25 rounds of 16384 keys 601 / 791 us, 3.1 of 32768 2787 / 3335, 6.1 of 40000
+//   6290 / 7050, 8.1 of 40000 7935 / 8640;
+//   prompts without anything before them, whose first rows are left over and see
+//   few keys: 1.2 rounds 78 / 71 us, 3.1 314 / 302, 6.1 1054 / 1043.
+// All of them are split alike, by their number: which request is the long one is
+// not looked at.  A chunk of 200 over 32768 keys (16 heads on 2) takes 84 us alone
+// and 395 beside seven of 200 over 200.
 struct ManyShares {
   int total, whole, splits;  // row tiles; those (the last ones) that are not split
   __device__ __forceinline__ ManyShares(const AttendArgs& a, const ManyGrid& grid, int tiles) : total(tiles), whole(tiles), splits(1) {
     const int rounds = tiles * a.kv_heads / grid.round;  // fewer items than workgroups in the grid, below 2^31
-    if (rounds >= kManyRounds) return;
     const int left = tiles - rounds * grid.round / a.kv_heads;
     if (left <= 0) return;
     const int fit = grid.round / (left * a.kv_heads);
