@@ -433,9 +433,8 @@ int kvc_step_tables(kvc_stream_t stream, int n_seq, const int32_t* computed_toke
  * it, and never k or v, nor its own rows each other; turned keys and the values go
  * to row slot_mapping[t] of the cache ([num_pages][128][kv_heads][head_dim]); slots
  * outside [0, num_pages*128) store nothing.  A slot may be named by one token only,
- * and the two caches may not be one.
- * head_dim <= 1024, rotary_dim <= 512.  No counterpart in the reference (its host's
- * model does it). */
+ * and the two caches may not be one.  head_dim <= 1024, rotary_dim <= 512.  No
+ * counterpart in the reference (its host's model does it). */
 int kvc_rotate_and_store(kvc_stream_t stream, int dtype, int rope_style, int64_t num_tokens, int heads, int kv_heads,
                          int head_dim, int rotary_dim, const void* q, int64_t q_token_stride, int64_t q_head_stride,
                          const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
@@ -453,7 +452,7 @@ int kvc_rotate_and_store(kvc_stream_t stream, int dtype, int rope_style, int64_t
  * Places are physical: after a compaction the window counts kept tokens, and
  * sinks are the first kept ones (protected_prefix keeps a prompt's first).  Keys
  * in pages outside [0, num_pages) or past max_blocks are not seen; rows that see
- * no key give zeros; what a key's row holds never reaches a row that does not
+ * no key, or only scores of -infinity, give zeros; what a key's row holds never reaches a row that does not
  * see it, NaN and infinities included.  Query head h*qpk + g belongs to KV head
  * h.  Element (t, head, d) of q and out at t*token_stride + head*head_stride + d;
  * strides in multiples of 8 elements, every pointer 16-byte aligned, head_dim a

@@ -11,12 +11,12 @@
 // a SIMD's: one group forms a tile's weights between the products of the next
 // tile's scores.
 //
-// 2048 tokens (40 heads on 8, head_dim 128) over 16384 keys: 600 us, 1.07
-// PFLOP/s, a library product of 16384^3 1.58.  There the card's power is the
-// limit: the kernel needs 1.19 million cycles at 1.93 GHz, its simpler forms
-// 1.48 million at 2.19 GHz took hardly longer.  16 heads on 2: head_dim 64 311 us
-// of 4096 tokens (0.9 PFLOP/s, the softmax's), of 2048 head_dim 192 403 us (1.0)
-// and 256 593 us (0.9).
+// 2048 tokens (40 heads on 8, head_dim 128) over 16384 keys: 600 - 615 us, 1.05 -
+// 1.07 PFLOP/s, a library product of 16384^3 1.58.  The matrix cores are busy 52% of
+// the time, LDS 32%; 1.19 million cycles at 1.93 GHz, where simpler forms took 1.48
+// million at 2.19: the clock falls as the matrix cores fill.  16 heads on 2: head_dim
+// 64 311 us of 4096 tokens (0.9 PFLOP/s, the softmax's), of 2048 head_dim 192 390 us
+// (1.0) and 256 600 us (0.9).
 //
 // Scores are formed transposed (S^T = K Q^T, 32x32x16): a lane holds one row's
 // scores (its other half in lane ^ 32), so the softmax needs one exchange, and
@@ -25,7 +25,9 @@
 // + j%4.  Weights are rounded to the cache's 16-bit type for that product, and the
 // rounded ones are what is summed, so that a row's weights add up to one: what is
 // left is half a step of how far the values lie from their mean, where the output's
-// own rounding is half a step of it.  The maxima, sums and outputs are float32.
+// own rounding is half a step of it: bf16 outputs are 2.2e-3 off float64, 1.7e-3 with
+// a second word for each weight, which would take 821 us for 614 (head_dim 192 628
+// for 397, 256 754 for 601).  The maxima, sums and outputs are float32.
 
 #include <type_traits>
 #include <utility>

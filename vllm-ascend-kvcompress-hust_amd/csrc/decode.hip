@@ -100,10 +100,10 @@ __device__ __forceinline__ int32_t step_page(const int64_t* ids, int64_t count, 
 
 // Workgroup (r, share) writes request r's row of every table, the row's entries
 // and tokens spread over the shares; the workgroups behind the last request
-// write the padding tokens.  Each adds up the new tokens before its request
-// itself (a request's count is 4 bytes): no launch or wait between the sum and
-// its readers.  64 requests 3.6 us, 512 with 24 chunks among them 5.4: the
-// dependent loads, the tables' bytes take less than 1.
+// write the padding tokens.  Each adds up the new tokens of all requests before its
+// own itself (n^2 / 2 reads of 4 bytes a share, from L2): no launch or wait between
+// the sum and its readers.  64 requests 3.6 us, 512 with 24 chunks among them 5.3:
+// the dependent loads, the tables' bytes take less than 1.
 __global__ __launch_bounds__(kDecodeThreads) void step_tables_kernel(StepTables a) {
   __shared__ int64_t part[kDecodeThreads / 64];
   const int r = blockIdx.x / a.shares, share = blockIdx.x - r * a.shares;
