@@ -473,6 +473,29 @@ def test_small_weights_of_many_keys_add_up(hip_device, dim, heads, kv, new) -> N
     assert ((got - want).abs() <= bound).all(), (float(got.min()), float(got.max()), float(want.min()))
 
 
+@pytest.mark.parametrize("dim, heads, kv, new", [(64, 2, 2, 1), (64, 16, 2, 3), (64, 4, 2, 40), (128, 16, 2, 6), (192, 4, 2, 20), (256, 4, 2, 20)])
+def test_small_weights_count_in_the_sum(hip_device, dim, heads, kv, new) -> None:
+    """fp16: values of 1 give 1, whatever the weights: 131068 of 2^-23 to 2^-25 of
+    the largest, which the many-rows kernel holds below fp16's normal range, are
+    2^-9 of the sum.
+
+    Bounds.  Output: half a step, 2^-11.  Both sums are of the same rounded weights
+    (two words leave 2^-40 of the largest each, 2^-23 in all): what differs is
+    float32's rounding of 4096 products one after another, 2^-12 each."""
+    length = 131072
+    k = torch.zeros((length // 128, 128, kv, dim), dtype=FP16, device=hip_device)
+    g = torch.Generator(device=hip_device).manual_seed(dim)
+    k[..., 3] = -16 - 1.3 * torch.rand(k.shape[:3], generator=g, device=hip_device).half()
+    k[0, 5::32, :, 3] = 0.0
+    v = torch.ones_like(k)
+    q = torch.zeros((new, heads, dim), dtype=FP16, device=hip_device)
+    q[..., 3] = 1.0
+    d = lambda x: torch.tensor(x, dtype=torch.int32, device=hip_device)  # noqa: E731
+    table = torch.arange(length // 128, dtype=torch.int32, device=hip_device)[None]
+    got = _serving().attend_paged(q, k, v, d([0, new]), d([length]), table, scale=1.0, max_query_len=new, max_seq_len=1).double()
+    assert float((got - 1).abs().max()) <= 2.0**-11 + 2 * 2.0**-12
+
+
 @pytest.mark.parametrize("dim, new", [(64, 1), (128, 40), (192, 40), (256, 40)])
 def test_weights_of_huge_scores_stay_in_range(hip_device, dim, new) -> None:
     """fp16: scores of 2^27 + 16 and, in later tiles, one float32 step more, 16.  A
